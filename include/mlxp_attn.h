@@ -45,7 +45,9 @@ typedef enum mlxp_status {
 typedef enum mlxp_dtype {
   MLXP_DTYPE_FP32 = 0,
   MLXP_DTYPE_BF16 = 1,
-  MLXP_DTYPE_FP16 = 2
+  MLXP_DTYPE_FP16 = 2,
+  MLXP_DTYPE_E4M3 = 3, /* 8-bit paged caches only: mlxp_paged_append,  */
+  MLXP_DTYPE_INT8 = 4  /* mlxp_quant_paged_attn                        */
 } mlxp_dtype;
 
 /* Library version as MAJOR*10000 + MINOR*100 + PATCH. */
@@ -356,6 +358,123 @@ int mlxp_paged_attn(const void* q, const void* k_pool, const void* v_pool,
 size_t mlxp_paged_attn_workspace_size(int dtype, int64_t B, int64_t H, int64_t Sq, int64_t D,
                                       int64_t kv_heads, int64_t num_blocks, int64_t block_size,
                                       int64_t max_blocks, int64_t kv_splits);
+
+/*
+ * RMS norm of query and key head rows followed by the half-split rotation, one launch for both
+ * tensors.  With h = D / 2, r = (mean(x^2) + eps)^-1/2 and (c, s) the table row of the token's
+ * position: y = x * r * w; out[:h] = y[:h] c - y[h:] s, out[h:] = y[:h] s + y[h:] c.  The
+ * rotation is that of mlxp_rope; the norm has no counterpart in the reference.  Computed in fp32,
+ * rounded once.
+ *
+ * The calls below take one pointer to a host struct: a decode step's call then costs its caller
+ * little.  Every field is 8 bytes; `size` is sizeof the struct; unused pointers are NULL.
+ * Strides are element strides in (batch, head, seq) order; the dim stride is 1.  D is even and
+ * at most 256; any alignment of the elements is accepted, 16-byte aligned rows are faster.
+ */
+typedef struct mlxp_qk_norm_rope_args {
+  uint64_t size;
+  const void *q, *k;             /* [B][Hq][Sq][D], [B][Hk][Sk][D] */
+  void *q_out, *k_out;           /* forward: the results; backward: dq, dk */
+  const void *gq, *gk;           /* backward: gradients of the results; NULL skips that tensor */
+  const void *q_weight, *k_weight; /* [D], of their own dtypes; both or neither (no norm) */
+  void *dq_weight, *dk_weight;   /* backward: in the weights' dtypes; NULL: not wanted */
+  const float *cos_cache, *sin_cache; /* [n_pos][D / 2]; both or neither (no rotation) */
+  const int32_t* positions;      /* NULL: offset + sequence index.  Else the token's position, with
+                                    Sq == Sk: negative marks padding (zeros, no gradient), past
+                                    the tables gives NaN */
+  int64_t dtype, q_weight_dtype, k_weight_dtype;
+  int64_t B, Sq, Sk, Hq, Hk, D, n_pos, q_offset, k_offset;
+  int64_t pos_strides[2];        /* of positions: (batch, seq) */
+  int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3];
+  int64_t gq_strides[3], gk_strides[3];
+  double eps;
+  void* workspace;               /* backward: >= mlxp_qk_norm_rope_bwd_workspace_size bytes */
+  uint64_t ws_bytes;
+  void* stream;
+} mlxp_qk_norm_rope_args;
+
+int mlxp_qk_norm_rope(const mlxp_qk_norm_rope_args* args);
+
+/* Gradients of mlxp_qk_norm_rope: dq, dk and the weights' (summed in fp32 in a fixed order, so
+ * that they are the same every time). */
+int mlxp_qk_norm_rope_bwd(const mlxp_qk_norm_rope_args* args);
+
+/* Bytes of workspace mlxp_qk_norm_rope_bwd needs for head_dim D (16-byte aligned). */
+size_t mlxp_qk_norm_rope_bwd_workspace_size(int64_t D);
+
+/*
+ * New keys and values into a paged pool (the pools mlxp_paged_attn and mlxp_quant_paged_attn
+ * read), keys, and queries beside them, normed and rotated on the way: one launch.  Token i of
+ * sequence b (i < new_lens[b]) has position pos = context_lens[b] + i and goes to row
+ * pos % block_size of pool block block_tables[b][pos / block_size]; where the position is
+ * negative or past the table, or the block id outside [0, num_blocks), the token is dropped.
+ * Nothing else in the pools is written (an 8-bit block's earlier rows where its scale grows).
+ * q_out rows past new_lens or with a position outside [0, max_blocks * block_size) are zeros.
+ *
+ * cache_dtype: the inputs' dtype, or MLXP_DTYPE_E4M3 / MLXP_DTYPE_INT8, where one fp32 scale a
+ * (block, head) multiplies the codes.  A block whose first row is among the new tokens takes the
+ * least power of two s >= 2^-126 with amax <= qmax * s over its new tokens (finite values; qmax
+ * 448 or 127); a block that holds tokens already keeps its scale, or takes s where that is larger
+ * and its earlier codes are rescaled.  Codes are round-to-nearest-even of value / scale, clamped to +-qmax;
+ * NaN stays NaN in e4m3 and is 0 in int8.
+ *
+ * A block that receives tokens must be listed once: sequences may share only blocks that are full.
+ */
+typedef struct mlxp_paged_append_args {
+  uint64_t size;
+  const void *k, *v;             /* [B][Hk][S][D] */
+  const void* q;                 /* [B][Hq][S][D] or NULL */
+  void* q_out;
+  void *k_pool, *v_pool;         /* (num_blocks, block_size, Hk, D) through pool_strides */
+  float *k_scales, *v_scales;    /* (num_blocks, Hk) through scale_strides; 8-bit caches only */
+  const int32_t *block_tables, *context_lens;
+  const int32_t* new_lens;       /* [B] or NULL: S */
+  const void *q_weight, *k_weight; /* norm weights [D], each or NULL */
+  const float *cos_cache, *sin_cache; /* [n_pos][D / 2], n_pos >= max_blocks * block_size, or NULL */
+  int64_t dtype, cache_dtype, q_weight_dtype, k_weight_dtype;
+  int64_t B, S, Hq, Hk, D, num_blocks, block_size, max_blocks, bt_stride, n_pos;
+  int64_t k_strides[3], v_strides[3], q_strides[3], q_out_strides[3];
+  int64_t pool_strides[3];       /* (block, token, head), shared by both pools */
+  int64_t scale_strides[2];      /* (block, head), shared by both */
+  double eps;
+  void* stream;
+} mlxp_paged_append_args;
+
+int mlxp_paged_append(const mlxp_paged_append_args* args);
+
+/*
+ * Attention over a paged cache of 8-bit codes and one fp32 scale a (block, head).  The queries of
+ * sequence b are its last query_lens[b] positions: query i sits at context_lens[b] -
+ * query_lens[b] + i.  Key t counts when t < context_lens[b], its slot's id is in
+ * [0, num_blocks), t <= the query's position if causal, and it is within `window` positions of
+ * the query (before it; both sides when not causal).  ALiBi adds slope[h] * (t - position).
+ * A query without keys, and rows past query_lens, are zeros.  q and o: fp32, bf16 or fp16, rows
+ * 16-byte aligned; pools 16-byte aligned with strides that are multiples of 16; D 32, 64 or 128.
+ * Scales are taken as of magnitude 2^-100 to 2^100.
+ */
+typedef struct mlxp_quant_paged_attn_args {
+  uint64_t size;
+  const void* q;                 /* [B][H][Sq][D] */
+  void* o;
+  const void *k_pool, *v_pool;   /* (num_blocks, block_size, kv_heads, D) codes */
+  const float *k_scales, *v_scales; /* (num_blocks, kv_heads) */
+  const int32_t *block_tables, *context_lens;
+  const int32_t* query_lens;     /* [B] or NULL: Sq */
+  const float* alibi_slopes;     /* [H] or NULL */
+  int64_t dtype, cache_dtype;
+  int64_t B, Sq, H, kv_heads, D, num_blocks, block_size, max_blocks, bt_stride;
+  int64_t causal, window;        /* window: -1 = none */
+  int64_t q_strides[3], o_strides[3], pool_strides[3], scale_strides[2];
+  double scale;
+  void* workspace;               /* >= mlxp_quant_paged_attn_workspace_size, 256-byte aligned */
+  uint64_t ws_bytes;
+  void* stream;
+} mlxp_quant_paged_attn_args;
+
+int mlxp_quant_paged_attn(const mlxp_quant_paged_attn_args* args);
+
+/* Bytes of workspace mlxp_quant_paged_attn needs on the current device (0 for invalid shapes). */
+size_t mlxp_quant_paged_attn_workspace_size(const mlxp_quant_paged_attn_args* args);
 
 /*
  * Device-side status word of the current device: 0 when every bounded wait completed,

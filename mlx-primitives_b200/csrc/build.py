@@ -9,6 +9,7 @@ travels with the source tree; the Python shim loads it from there (or from $MLXP
 from __future__ import annotations
 
 import argparse
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -19,8 +20,9 @@ CSRC = Path(__file__).resolve().parent
 PKG_ROOT = CSRC.parent
 INCLUDE = PKG_ROOT.parent / "include"
 OUT = PKG_ROOT / "mlx_primitives" / "libmlxp_attn.so"
-SOURCES = [CSRC / "mlxp_attn.cu"]
-DEPS = SOURCES + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "mlxp_attn.h"]
+SOURCES = [CSRC / "mlxp_attn.cu", CSRC / "mlxp_cache.cu", CSRC / "mlxp_quant.cu"]
+DEPS = SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [INCLUDE / "mlxp_attn.h"]
+OBJ = CSRC / "_build"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -31,17 +33,21 @@ def nvcc_path() -> str:
     raise RuntimeError("nvcc not found (set $NVCC)")
 
 
-def command(debug: bool = False, verbose_ptxas: bool = False) -> list[str]:
-    cmd = [nvcc_path(), *ARCH, "-std=c++17", "-O3", "-lineinfo", "-shared",
-           "-Xcompiler", "-fPIC", "-cudart", "shared",
-           "-Xlinker", "-rpath,/usr/local/cuda/lib64",
-           "-I", str(INCLUDE), "-o", str(OUT), "-ldl"]
+def commands(debug: bool = False, verbose_ptxas: bool = False) -> tuple[list[list[str]], list[str]]:
+    """The compile command of every source (they run in parallel) and the link command."""
+    nvcc = nvcc_path()
+    flags = [*ARCH, "-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-cudart", "shared",
+             "-I", str(INCLUDE)]
     if debug:
-        cmd += ["-DMLXP_DEBUG_CHECKS=1"]
+        flags += ["-DMLXP_DEBUG_CHECKS=1"]
     if verbose_ptxas:
-        cmd += ["-Xptxas", "-v"]
-    cmd += [str(s) for s in SOURCES]
-    return cmd
+        flags += ["-Xptxas", "-v"]
+    objects = [OBJ / (s.stem + ".o") for s in SOURCES]
+    compiles = [[nvcc, *flags, "-c", str(s), "-o", str(o)] for s, o in zip(SOURCES, objects)]
+    link = [nvcc, *ARCH, "-shared", "-cudart", "shared",
+            "-Xlinker", "-rpath,/usr/local/cuda/lib64", "-o", str(OUT), "-ldl",
+            *map(str, objects)]
+    return compiles, link
 
 
 def up_to_date() -> bool:
@@ -54,12 +60,19 @@ def up_to_date() -> bool:
 def build(force: bool = False, debug: bool = False, verbose_ptxas: bool = False) -> Path:
     if not force and not debug and not verbose_ptxas and up_to_date():
         return OUT
-    cmd = command(debug=debug, verbose_ptxas=verbose_ptxas)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
-    if verbose_ptxas:
-        sys.stderr.write(res.stderr)
+    compiles, link = commands(debug=debug, verbose_ptxas=verbose_ptxas)
+    OBJ.mkdir(exist_ok=True)
+
+    def run(cmd):
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+        if verbose_ptxas:
+            sys.stderr.write(res.stderr)
+
+    with concurrent.futures.ThreadPoolExecutor() as pool:
+        list(pool.map(run, compiles))
+    run(link)
     return OUT
 
 

@@ -1,0 +1,18 @@
+// host_common.h — what the library's translation units share on the host: the thread's error
+// message and the per-device lookups (defined in mlxp_attn.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#define MLXP_INTERNAL __attribute__((visibility("hidden")))
+
+namespace mlxp {
+
+// Records the message of mlxp_last_error and returns `code`.
+MLXP_INTERNAL int fail(int code, const char* fmt, ...);
+MLXP_INTERNAL int cuda_fail(cudaError_t e, const char* what);
+MLXP_INTERNAL int current_device(int& dev);
+// Device status word and SM count of the current device; either may be null.
+MLXP_INTERNAL int device_info(int** status, int* sms);
+
+}  // namespace mlxp

@@ -20,6 +20,7 @@
 
 #include "../../include/mlxp_attn.h"
 #include "attn_common.cuh"
+#include "host_common.h"
 #include "attn_fwd_fp32.cuh"
 #include "attn_fwd_sm100.cuh"
 #include "rope.cuh"
@@ -40,6 +41,8 @@ namespace {
 
 thread_local std::string t_last_error;
 
+}  // namespace
+
 int fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
@@ -54,6 +57,8 @@ int cuda_fail(cudaError_t e, const char* what) {
   return fail(MLXP_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
+namespace {
+
 std::atomic<unsigned long long> g_timeout_ns{2000000000ull};
 // Test hook (mlxp_set_backward_path): 1 = always the CUDA-core backward.
 std::atomic<int> g_bwd_force_cuda_cores{0};
@@ -65,6 +70,8 @@ unsigned* g_counter_ptr[kMaxDevices] = {};
 std::atomic<unsigned> g_counter_seq[kMaxDevices];
 int g_num_sms[kMaxDevices] = {};
 unsigned long long g_attr_done[kMaxDevices] = {};
+
+}  // namespace
 
 int current_device(int& dev) {
   cudaError_t e = cudaGetDevice(&dev);
@@ -96,6 +103,8 @@ int device_info(int** status, int* sms) {
   if (sms) *sms = g_num_sms[dev];
   return MLXP_OK;
 }
+
+namespace {
 
 // Sets the dynamic shared memory limit of a kernel once per device.
 template <typename K>

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -17,7 +18,7 @@ import torch
 
 __all__ = [
     "MLXP_OK", "MLXP_ERR_INVALID", "MLXP_ERR_UNSUPPORTED", "MLXP_ERR_TIMEOUT",
-    "DTYPE_CODES", "lib", "lib_path", "check", "EXPORTED_SYMBOLS",
+    "DTYPE_CODES", "CACHE_DTYPE_CODES", "ArgStruct", "lib", "lib_path", "check", "EXPORTED_SYMBOLS",
 ]
 
 MLXP_OK = 0
@@ -29,6 +30,8 @@ MLXP_ERR_TIMEOUT = 5
 MLXP_ERR_WORKSPACE = 6
 
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+# element types of 8-bit paged caches
+CACHE_DTYPE_CODES = {torch.float8_e4m3fn: 3, torch.int8: 4}
 
 _i64 = ctypes.c_int64
 _p = ctypes.c_void_p
@@ -101,6 +104,13 @@ _SIGNATURES = {
         _p, _p, _p, _p, _p, ctypes.c_int, _i64, _i64, _i64, _i64,
         _i64x4, _i64x4, _i64x4, _i64x4, ctypes.c_float, _p, ctypes.c_size_t, _p]),
     "mlxp_ring_destroy": (ctypes.c_int, [_p]),
+    # these take one packed argument struct (ArgStruct below)
+    "mlxp_qk_norm_rope": (ctypes.c_int, [ctypes.c_char_p]),
+    "mlxp_qk_norm_rope_bwd": (ctypes.c_int, [ctypes.c_char_p]),
+    "mlxp_qk_norm_rope_bwd_workspace_size": (ctypes.c_size_t, [_i64]),
+    "mlxp_paged_append": (ctypes.c_int, [ctypes.c_char_p]),
+    "mlxp_quant_paged_attn": (ctypes.c_int, [ctypes.c_char_p]),
+    "mlxp_quant_paged_attn_workspace_size": (ctypes.c_size_t, [ctypes.c_char_p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -163,3 +173,48 @@ def strides4(t: torch.Tensor, layout: str) -> ctypes.Array:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class ArgStruct:
+    """Packer of one of the header's argument structs: n fields of 8 bytes, integers and pointers
+    but for the doubles at the indices `doubles`.  ``pack(*fields)`` gives the bytes the C
+    function reads; the leading ``size`` field, by which it checks the layout, is put there."""
+
+    def __init__(self, n: int, doubles: tuple = ()):
+        fmt = "".join("d" if i in doubles else "q" for i in range(n))
+        self._struct = struct.Struct("=" + fmt)
+        self.size = self._struct.size
+
+    def pack(self, *fields) -> bytes:
+        return self._struct.pack(self.size, *fields)
+
+
+def seq_strides(t: torch.Tensor) -> tuple:
+    """Element strides (batch, head, seq) of a (batch, seq, head, dim) tensor."""
+    s = t.stride()
+    return s[0], s[2], s[1]
+
+
+def address(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def raw_stream(device: torch.device) -> int:
+    """Handle of the device's current stream, without building a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _NoSwitch:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_SWITCH = _NoSwitch()
+
+
+def on_device(device: torch.device):
+    """Context in which `device` is the current device; free of cost where it already is."""
+    return _NO_SWITCH if torch.cuda.current_device() == device.index else torch.cuda.device(device)
