@@ -131,7 +131,7 @@ enum : int {
   kSiteMmaP = 3,
   kSiteSoftmaxS = 4,
   kSiteSoftmaxO = 5,
-  kSiteDrain = 6,
+  // 6: kSiteDrain (sm100_ptx.cuh)
   kSiteSelfTest = 7,
   kSiteWork = 8,
   kSiteEpilogue = 10,
@@ -151,16 +151,6 @@ enum : int {
 #endif
 template <int D>
 constexpr int kPolyPerOct = (D == 64) ? MLXP_POLY_D64 : MLXP_POLY_D128;
-
-// Wait without looking at the abort flag (used when draining after an abort).
-__device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity, int* status,
-                                                uint64_t timeout_ns) {
-  int dummy_flag = 0;
-  WaitCtx w{&dummy_flag, status, timeout_ns};
-  if (mbar_try_wait(bar, parity)) return true;
-  // mbar_wait_slow reads the flag through a volatile pointer; a private flag is never set.
-  return mbar_wait_slow(bar, parity, w, kSiteDrain);
-}
 
 __device__ __forceinline__ void tma_coords(const TmaCoordMap& cm, int s, int h, int b, int& c1,
                                            int& c2, int& c3) {

@@ -2,7 +2,9 @@
 // message and the per-device lookups (defined in mlxp_attn.cu).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>
 
 #define MLXP_INTERNAL __attribute__((visibility("hidden")))
 
@@ -14,5 +16,10 @@ MLXP_INTERNAL int cuda_fail(cudaError_t e, const char* what);
 MLXP_INTERNAL int current_device(int& dev);
 // Device status word and SM count of the current device; either may be null.
 MLXP_INTERNAL int device_info(int** status, int* sms);
+
+// The driver's tensor-map encoder.
+MLXP_INTERNAL int tensor_map_encoder(PFN_cuTensorMapEncodeTiled_v12000* fn);
+// Limit of every bounded device-side wait (mlxp_set_wait_timeout_ns).
+MLXP_INTERNAL unsigned long long wait_timeout_ns();
 
 }  // namespace mlxp

@@ -143,6 +143,18 @@ int get_encode_fn() {
   return MLXP_OK;
 }
 
+}  // namespace
+
+int tensor_map_encoder(PFN_cuTensorMapEncodeTiled_v12000* fn) {
+  if (int rc = get_encode_fn()) return rc;
+  *fn = g_encode;
+  return MLXP_OK;
+}
+
+unsigned long long wait_timeout_ns() { return g_timeout_ns.load(); }
+
+namespace {
+
 // Builds a 4-D tensor map over a (b, h, s, d)-strided tensor with a box of 64 d-elements by
 // `box_rows` s-rows.  The three outer dims are ordered by stride so that the map is monotonic
 // whatever the layout (BHSD: s,h,b; BSHD: h,s,b); size-1 and stride-0 (broadcast) dims are

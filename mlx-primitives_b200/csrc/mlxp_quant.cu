@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "../../include/mlxp_attn.h"
@@ -26,9 +27,9 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 // CTAs an SM holds, from the kernels' registers (the launch bounds below are the same numbers).
 template <int D, int NT, bool SPLIT>
 constexpr int qa_min_ctas() {
-  if (SPLIT) return D == 128 ? 2 : 3;
-  if (NT == 2) return D == 128 ? 2 : 3;
-  return D == 128 ? 3 : 4;
+  if (SPLIT) return D == 128 ? 2 : 4;
+  if (NT == 2) return D == 128 ? 3 : 4;
+  return 4;
 }
 
 int qa_ctas(int64_t dtype, int64_t D, int nt) {
@@ -91,11 +92,52 @@ QaPlan qa_plan(const mlxp_quant_paged_attn_args* a, int sms, QaParams& p) {
   return n;
 }
 
+// Tensor maps of the pools, {D, heads, block_size, blocks} with boxes of one head's 16 rows.
+struct QaMaps {
+  CUtensorMap k, v;
+  bool use;  // a tile of 16 keys lies in one block, and the pools suit TMA
+};
+
+int qa_maps(const mlxp_quant_paged_attn_args* a, QaMaps& m) {
+  m.use = false;
+  if (a->block_size % kQaTile || a->num_blocks < 1) return MLXP_OK;
+  int64_t sb = a->pool_strides[0], st = a->pool_strides[1], sh = a->pool_strides[2];
+  if (a->kv_heads == 1) sh = a->D;                 // strides that no coordinate uses
+  if (a->num_blocks == 1) sb = st * a->block_size;
+  for (const int64_t x : {sb, st, sh})
+    if (x <= 0 || x % 16 || x >= (int64_t(1) << 40)) return MLXP_OK;
+  PFN_cuTensorMapEncodeTiled_v12000 encode;
+  if (int rc = tensor_map_encoder(&encode)) return rc;
+  const cuuint64_t dims[4] = {(cuuint64_t)a->D, (cuuint64_t)a->kv_heads, (cuuint64_t)a->block_size,
+                              (cuuint64_t)a->num_blocks};
+  const cuuint64_t strides[3] = {(cuuint64_t)sh, (cuuint64_t)st, (cuuint64_t)sb};
+  const cuuint32_t box[4] = {(cuuint32_t)a->D, 1, (cuuint32_t)kQaTile, 1}, ones[4] = {1, 1, 1, 1};
+  const CUtensorMapSwizzle swizzle = a->D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : a->D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+  for (int i = 0; i < 2; ++i)
+    if (encode(i ? &m.v : &m.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(i ? a->v_pool : a->k_pool),
+               dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return MLXP_OK;
+  m.use = true;
+  return MLXP_OK;
+}
+
 template <typename T, int D, int NT, bool INT8, bool BS16>
-int qa_launch(const QaParams& p, const QaPlan& n, cudaStream_t s) {
-  quant_attn_kernel<T, D, NT, INT8, BS16, qa_min_ctas<D, NT, sizeof(T) == 4>()>
-      <<<(unsigned)n.grid, 32 * kQaWarps, 0, s>>>(p);
-  cudaError_t e = cudaGetLastError();
+int qa_launch(const QaMaps& maps, const QaParams& p, const QaPlan& n, cudaStream_t s) {
+  auto kernel = quant_attn_kernel<T, D, NT, INT8, BS16, qa_min_ctas<D, NT, sizeof(T) == 4>()>;
+  constexpr int smem = qa_smem_bytes<D, NT, BS16>();
+  static std::atomic<unsigned long long> attr_done{0};  // one bit per device
+  int dev;
+  if (int rc = current_device(dev)) return rc;
+  cudaError_t e;
+  if (!(attr_done.load() >> dev & 1ull)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(quantized paged attention)");
+    attr_done.fetch_or(1ull << dev);
+  }
+  kernel<<<(unsigned)n.grid, 32 * kQaWarps, smem, s>>>(maps.k, maps.v, p);
+  e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "quantized paged attention launch");
   if (n.grid == 1) return MLXP_OK;
   cudaLaunchConfig_t cfg{};
@@ -112,24 +154,23 @@ int qa_launch(const QaParams& p, const QaPlan& n, cudaStream_t s) {
 }
 
 template <typename T, int D, int NT>
-int qa_launch_n(const QaParams& p, const QaPlan& n, bool int8, cudaStream_t s) {
-  const bool bs16 = p.block_size % kQaTile == 0;
-  if (int8) return bs16 ? qa_launch<T, D, NT, true, true>(p, n, s) : qa_launch<T, D, NT, true, false>(p, n, s);
-  return bs16 ? qa_launch<T, D, NT, false, true>(p, n, s) : qa_launch<T, D, NT, false, false>(p, n, s);
+int qa_launch_n(const QaMaps& m, const QaParams& p, const QaPlan& n, bool int8, cudaStream_t s) {
+  if (int8) return m.use ? qa_launch<T, D, NT, true, true>(m, p, n, s) : qa_launch<T, D, NT, true, false>(m, p, n, s);
+  return m.use ? qa_launch<T, D, NT, false, true>(m, p, n, s) : qa_launch<T, D, NT, false, false>(m, p, n, s);
 }
 
 template <typename T, int D>
-int qa_launch_d(const QaParams& p, const QaPlan& n, bool int8, cudaStream_t s) {
+int qa_launch_d(const QaMaps& m, const QaParams& p, const QaPlan& n, bool int8, cudaStream_t s) {
   if constexpr (sizeof(T) == 2)
-    if (n.nt == 2) return qa_launch_n<T, D, 2>(p, n, int8, s);
-  return qa_launch_n<T, D, 1>(p, n, int8, s);
+    if (n.nt == 2) return qa_launch_n<T, D, 2>(m, p, n, int8, s);
+  return qa_launch_n<T, D, 1>(m, p, n, int8, s);
 }
 
 template <typename T>
-int qa_launch_t(int64_t D, const QaParams& p, const QaPlan& n, bool int8, cudaStream_t s) {
-  if (D == 128) return qa_launch_d<T, 128>(p, n, int8, s);
-  if (D == 64) return qa_launch_d<T, 64>(p, n, int8, s);
-  return qa_launch_d<T, 32>(p, n, int8, s);
+int qa_launch_t(int64_t D, const QaMaps& m, const QaParams& p, const QaPlan& n, bool int8, cudaStream_t s) {
+  if (D == 128) return qa_launch_d<T, 128>(m, p, n, int8, s);
+  if (D == 64) return qa_launch_d<T, 64>(m, p, n, int8, s);
+  return qa_launch_d<T, 32>(m, p, n, int8, s);
 }
 
 }  // namespace
@@ -168,9 +209,13 @@ int mlxp_quant_paged_attn(const mlxp_quant_paged_attn_args* a) {
       return fail(MLXP_ERR_INVALID, "q and o rows must start on 16 bytes");
     if (a->pool_strides[d] % 16) return fail(MLXP_ERR_INVALID, "pool strides must be multiples of 16");
   }
-  int sms;
-  if (int rc = device_info(nullptr, &sms)) return rc;
+  int sms, *status;
+  if (int rc = device_info(&status, &sms)) return rc;
+  QaMaps maps{};
+  if (int rc = qa_maps(a, maps)) return rc;
   QaParams p{};
+  p.status = status;
+  p.timeout_ns = wait_timeout_ns();
   const QaPlan n = qa_plan(a, sms, p);
   if (!a->workspace || a->ws_bytes < n.bytes())
     return fail(MLXP_ERR_WORKSPACE, "quantized paged attention needs %zu bytes of workspace, got %llu",
@@ -207,13 +252,14 @@ int mlxp_quant_paged_attn(const mlxp_quant_paged_attn_args* a) {
   p.block_size = (int)a->block_size;
   p.max_blocks = (int)a->max_blocks;
   p.causal = a->causal ? 1 : 0;
+  p.bs_pow2 = (p.block_size & (p.block_size - 1)) == 0;
   p.window = a->window;
   p.scale_log2 = (float)(a->scale * 1.4426950408889634);
   const bool int8 = a->cache_dtype == MLXP_DTYPE_INT8;
   const cudaStream_t s = (cudaStream_t)a->stream;
-  if (a->dtype == MLXP_DTYPE_BF16) return qa_launch_t<__nv_bfloat16>(a->D, p, n, int8, s);
-  if (a->dtype == MLXP_DTYPE_FP16) return qa_launch_t<__half>(a->D, p, n, int8, s);
-  return qa_launch_t<float>(a->D, p, n, int8, s);
+  if (a->dtype == MLXP_DTYPE_BF16) return qa_launch_t<__nv_bfloat16>(a->D, maps, p, n, int8, s);
+  if (a->dtype == MLXP_DTYPE_FP16) return qa_launch_t<__half>(a->D, maps, p, n, int8, s);
+  return qa_launch_t<float>(a->D, maps, p, n, int8, s);
 }
 
 }  // extern "C"

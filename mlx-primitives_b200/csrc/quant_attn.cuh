@@ -15,12 +15,15 @@
 // query rows as M = 16.  (tcgen05 needs M >= 64 rows and its operands in shared memory or TMEM,
 // which one query row cannot fill.)
 //
-// No shared memory on the way.  The order of a dot product's terms is free, so the fragment
-// layouts are chosen such that the bytes a lane loads are the bytes its fragments need: of a K
-// row the four lanes c of a row group hold 16-byte pieces c and, for D = 128, 4 + c, each word of
-// which is one k16 step's two pairs; of a V row the eight lanes g hold D / 8 bytes each, and a
-// byte permute of two keys' words gives the pairs along keys.  A warp loads the next tile into
-// registers while it computes on this one.
+// How the codes get there.  Where the block size is a multiple of 16 a tile is one TMA box of K
+// and one of V (16 rows of one head), three or four stages in flight a warp, each on its own
+// mbarrier: 87 % of the measured HBM rate at four contexts of 128K tokens.  Loads into registers
+// (257 us there against 190) left a warp one tile ahead, and cp.async (284 us) kept the load
+// path busy with 28 instructions a tile.  Other block sizes do take cp.async, every lane copying
+// the bytes that it reads itself.  The order of a dot product's terms is free, so the fragments
+// are filled straight from the rows: of a K row the four lanes c of a row group hold 16-byte
+// pieces, each word of which is one k16 step's two pairs; of a V row the eight lanes g hold
+// D / 8 bytes each, and a byte permute of two keys' words gives the pairs along keys.
 //
 // Precision.  16-bit queries are scaled by a power of two a row to [1, 2) at most and held in
 // fp16 (bf16 values lose nothing but below 2^-25 of the row's largest); fp32 queries and
@@ -54,6 +57,7 @@ constexpr int kQaWarps = 4;
 constexpr int kQaChunk = 64;   // keys a chunk
 constexpr int kQaTile = 16;    // keys a tile
 constexpr float kQaPScale = 32768.f;
+constexpr int kSiteQuantPaged = 12;  // device-status site of this kernel's waits
 
 struct QaPartInfo {  // written by every CTA: the unit its range starts inside of
   int v, hg;         // v = -1: it starts at a unit's first chunk (or has no chunks)
@@ -81,9 +85,11 @@ struct QaParams {
   int rows;                       // rows of a tile that exist anywhere: min(R, 8 NT)
   int RT, HP, HG;                 // row tiles, heads a unit, units a virtual sequence
   int num_blocks, block_size, max_blocks;
-  int causal;
+  int causal, bs_pow2;            // bs_pow2: the block size is a power of two
   long long window;               // -1: none
   float scale_log2;
+  int* status;                    // device status word (bounded waits)
+  unsigned long long timeout_ns;
 };
 
 // Keys of a virtual sequence.
@@ -142,6 +148,16 @@ __device__ __forceinline__ void qa_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same without a sum to add to.
+__device__ __forceinline__ void qa_mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 __device__ __forceinline__ uint32_t qa_transpose(uint32_t a) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -176,29 +192,6 @@ __device__ __forceinline__ float2 qa_unpack(uint32_t u) {
   return __half22float2(reinterpret_cast<const __half2&>(u));
 }
 
-template <int W>
-__device__ __forceinline__ void qa_ldg(const unsigned char* p, bool on, uint32_t* w) {
-#pragma unroll
-  for (int i = 0; i < W; ++i) w[i] = 0;
-  if (!on) return;
-  if constexpr (W % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < W / 4; ++i) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
-      w[4 * i] = u.x;
-      w[4 * i + 1] = u.y;
-      w[4 * i + 2] = u.z;
-      w[4 * i + 3] = u.w;
-    }
-  } else if constexpr (W == 2) {
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-    w[0] = u.x;
-    w[1] = u.y;
-  } else {
-    w[0] = __ldg(reinterpret_cast<const unsigned*>(p));
-  }
-}
-
 // Elements of a K row held by lane c as 4-byte words: words j < D/16, dims qa_kdim(j, c)..+3.
 template <int D>
 __device__ __forceinline__ int qa_kdim(int j, int c) {
@@ -206,133 +199,148 @@ __device__ __forceinline__ int qa_kdim(int j, int c) {
   return (j / 4) * 64 + 16 * c + 4 * (j % 4);
 }
 
+// A warp's ring of tiles in shared memory: 16 K rows, then 16 V rows, of D bytes, 16-byte chunks
+// swizzled as the tensor maps' 128-, 64- or 32-byte swizzle does.  The fragments fix only which
+// rows and chunks meet, so the rows and dims that the lanes take are chosen against bank
+// conflicts: row group g works on key qa_key(g) and on the V dims of piece qa_piece(g).
 template <int D>
-struct QaTile {
-  static constexpr int KW = D / 16, VW = D / 32;
-  uint32_t k[2][KW];     // rows g, g + 8
-  uint32_t v[4][VW];     // keys 2c, 2c + 1, 2c + 8, 2c + 9; bytes [g * D / 8, +D / 8)
-  float ks0, ks1, vs0, vs1;  // scales of rows g, g + 8
-  int t0;
-  bool ok0, ok1;         // rows g, g + 8 are keys in a pool block
+struct QaRing {
+  static constexpr int KW = D / 16, VW = D / 32;   // words a lane holds of a K row, a V row
+  static constexpr int KB = D == 32 ? 8 : 16, KP = 4 * KW / KB, VB = D / 8;
+  static constexpr int kHalf = kQaTile * D, kTileBytes = 2 * kHalf;
+  static constexpr int kStages = D == 128 ? 3 : 4;
+  // a warp's rows' scales and validity a stage, where the block size is not a multiple of 16
+  static constexpr int kMeta = 32 * 20;
+  static constexpr int kRing = kStages * kTileBytes;
 };
 
-// BS16: the block size is a multiple of 16, so that a tile lies in one block.
-template <int D, bool BS16>
-__device__ __forceinline__ void qa_load(const QaParams& p, const int* bt, long long head_off,
-                                        long long head_sc, int t0, int kend, int g, int c,
-                                        QaTile<D>& t) {
-  constexpr int KW = QaTile<D>::KW, VW = QaTile<D>::VW;
-  t.t0 = t0;
-  auto locate = [&](int key, bool in, int& id, long long& off) {
-    id = -1;
-    off = 0;
-    if (!in) return;
-    const unsigned slot = (unsigned)key / (unsigned)p.block_size;
-    const int got = __ldg(bt + slot);
-    if (got >= 0 && got < p.num_blocks) {
-      id = got;
-      off = (long long)got * p.p_sb + (long long)(key - (int)slot * p.block_size) * p.p_st + head_off;
-    }
-  };
-  int id0, id1;
-  long long o0, o1, ov[4];
-  bool okv[4];
-  if constexpr (BS16) {
-    locate(t0, t0 < kend, id0, o0);
-    id1 = id0;
-    t.ok0 = id0 >= 0 && t0 + g < kend;
-    t.ok1 = id0 >= 0 && t0 + g + 8 < kend;
+__device__ __forceinline__ int qa_key(int g) { return (g & 1) << 2 | g >> 1; }
+
+template <int D>
+__device__ __forceinline__ int qa_piece(int g) {
+  if constexpr (D == 128) return qa_key(g);
+  if constexpr (D == 64) return (g & 1) | (g & 2) << 1 | (g & 4) >> 1;
+  return g;
+}
+
+template <int D>
+__device__ __forceinline__ uint32_t qa_swizzle(uint32_t off) {
+  return off ^ ((off >> 7) & (D / 16 - 1)) << 4;
+}
+
+// The lane's places in a tile: K row qa_key(g) (row + 8: 8 D bytes on), V rows c and c + 4 (+ 8).
+template <int D>
+struct QaLane {
+  uint32_t k[QaRing<D>::KP], v[2];
+  __device__ __forceinline__ QaLane(int g, int c) {
+    using Q = QaRing<D>;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = 2 * c + (e & 1) + (e >> 1) * 8;
-      okv[e] = id0 >= 0 && t0 + r < kend;
-      ov[e] = o0 + r * p.p_st;
-    }
-    o1 = o0 + (g + 8) * p.p_st;
-    o0 += g * p.p_st;
-  } else {
-    locate(t0 + g, t0 + g < kend, id0, o0);
-    locate(t0 + g + 8, t0 + g + 8 < kend, id1, o1);
-    t.ok0 = id0 >= 0;
-    t.ok1 = id1 >= 0;
+    for (int i = 0; i < Q::KP; ++i) k[i] = qa_swizzle<D>(qa_key(g) * D + Q::KB * c + 64 * i);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = t0 + 2 * c + (e & 1) + (e >> 1) * 8;
-      int id;
-      locate(r, r < kend, id, ov[e]);
-      okv[e] = id >= 0;
-    }
+    for (int e = 0; e < 2; ++e) v[e] = Q::kHalf + qa_swizzle<D>((c + 4 * e) * D + Q::VB * qa_piece<D>(g));
   }
-  if constexpr (D == 128) {
-    qa_ldg<4>(p.k_pool + o0 + 16 * c, t.ok0, t.k[0]);
-    qa_ldg<4>(p.k_pool + o0 + 64 + 16 * c, t.ok0, t.k[0] + 4);
-    qa_ldg<4>(p.k_pool + o1 + 16 * c, t.ok1, t.k[1]);
-    qa_ldg<4>(p.k_pool + o1 + 64 + 16 * c, t.ok1, t.k[1] + 4);
-  } else {
-    qa_ldg<KW>(p.k_pool + o0 + 4 * KW * c, t.ok0, t.k[0]);
-    qa_ldg<KW>(p.k_pool + o1 + 4 * KW * c, t.ok1, t.k[1]);
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) qa_ldg<VW>(p.v_pool + ov[e] + g * (D / 8), okv[e], t.v[e]);
-  t.ks0 = t.ok0 ? __ldg(p.k_scales + id0 * p.sc_sb + head_sc) : 0.f;
-  t.ks1 = t.ok1 ? __ldg(p.k_scales + id1 * p.sc_sb + head_sc) : 0.f;
-  t.vs0 = t.ok0 ? __ldg(p.v_scales + id0 * p.sc_sb + head_sc) : 0.f;
-  t.vs1 = t.ok1 ? __ldg(p.v_scales + id1 * p.sc_sb + head_sc) : 0.f;
+};
+
+template <int N>
+__device__ __forceinline__ void qa_copy(uint32_t dst, const unsigned char* src, bool on) {
+  const int n = on ? N : 0;  // the rest is filled with zeros
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(N) : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void qa_lds(uint32_t src, uint32_t* w) {
+  if constexpr (N == 16)
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src) : "memory");
+  else if constexpr (N == 8)
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(src) : "memory");
+  else
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(src) : "memory");
 }
 
 // The state of a warp's rows: lane (g, c) holds query rows 2c, 2c + 1 of each n-tile.
 template <int D, int NT>
 struct QaState {
-  float acc[NT][D / 16][4];  // dims g * D/8 + 2t (0: row 2c, 1: row 2c + 1) and + 2t + 1 (2, 3)
+  float acc[NT][D / 16][4];  // dims qa_piece(g) * D/8 + 2t (0: row 2c, 1: row 2c + 1), + 2t + 1 (2, 3)
   float m[NT][2], l[NT][2];  // l: this lane's keys only, until the end
 };
 
+// Scales of the lane's K rows (keys qa_key(g), + 8) and log2 of |V's|, and whether they, and
+// the lane's V rows (keys c, c + 4, c + 8, c + 12), are keys in a block.
+struct QaRows {
+  float ks0, ks1, vs0, vs1, lv0, lv1;
+  bool ok0, ok1, okv[4];
+};
+
+__device__ __forceinline__ float qa_log_scale(float vs) {
+  return fminf(fmaxf(__log2f(fabsf(vs)), -100.f), 100.f);
+}
+
 template <int D, int NT, bool SPLIT, bool INT8>
-__device__ __forceinline__ void qa_step(const QaTile<D>& t, const uint32_t (&qf)[SPLIT ? 2 : 1][NT][D / 16][2],
+__device__ __forceinline__ void qa_step(uint32_t stage, const QaLane<D>& at, const QaRows& t, int t0,
+                                        const uint32_t (&qf)[SPLIT ? 2 : 1][NT][D / 16][2],
                                         const float (&qs)[NT][2], const int* row_lo,
                                         const int* row_hi, const float* row_slope,
                                         const int* row_pos, bool masked, int g, int c,
                                         QaState<D, NT>& st) {
-  constexpr int KW = D / 16, VW = D / 32;
+  using Q = QaRing<D>;
   float sa[NT][4], sb[NT][4];
+#pragma unroll
+  for (int i = 0; i < Q::KP; ++i) {
+    uint32_t k0[Q::KB / 4], k1[Q::KB / 4];
+    qa_lds<Q::KB>(stage + at.k[i], k0);
+    qa_lds<Q::KB>(stage + at.k[i] + 8 * D, k1);
+#pragma unroll
+    for (int x = 0; x < Q::KB / 4; ++x) {
+      const int j = i * (Q::KB / 4) + x;
+      uint32_t a0, a1, a2, a3;
+      qa_codes<INT8>(k0[x], a0, a2);
+      qa_codes<INT8>(k1[x], a1, a3);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {  // two chains of sums: even and odd words
+        float(&d)[4] = j & 1 ? sb[n] : sa[n];
+        if (j < 2) qa_mma0(d, a0, a1, a2, a3, qf[0][n][j][0], qf[0][n][j][1]);
+        else qa_mma(d, a0, a1, a2, a3, qf[0][n][j][0], qf[0][n][j][1]);
+        if constexpr (SPLIT) qa_mma(d, a0, a1, a2, a3, qf[1][n][j][0], qf[1][n][j][1]);
+      }
+    }
+  }
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sa[n][e] = sb[n][e] = 0.f;
+    for (int e = 0; e < 4; ++e) sa[n][e] = (sa[n][e] + sb[n][e]) * (qs[n][e & 1] * (e < 2 ? t.ks0 : t.ks1));
+  if (row_slope) {
 #pragma unroll
-  for (int j = 0; j < KW; ++j) {
-    uint32_t a0, a1, a2, a3;
-    qa_codes<INT8>(t.k[0][j], a0, a2);
-    qa_codes<INT8>(t.k[1][j], a1, a3);
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      qa_mma(j & 1 ? sb[n] : sa[n], a0, a1, a2, a3, qf[0][n][j][0], qf[0][n][j][1]);
-      if constexpr (SPLIT) qa_mma(j & 1 ? sa[n] : sb[n], a0, a1, a2, a3, qf[1][n][j][0], qf[1][n][j][1]);
-    }
+      for (int e = 0; e < 4; ++e) {
+        const int row = n * 8 + 2 * c + (e & 1);
+        sa[n][e] = fmaf(row_slope[row], (float)(t0 + qa_key(g) + (e < 2 ? 0 : 8) - row_pos[row]), sa[n][e]);
+      }
   }
-  const float lv0 = fminf(fmaxf(__log2f(fabsf(t.vs0)), -100.f), 100.f);
-  const float lv1 = fminf(fmaxf(__log2f(fabsf(t.vs1)), -100.f), 100.f);
+  if (masked) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = n * 8 + 2 * c + (e & 1), key = t0 + qa_key(g) + (e < 2 ? 0 : 8);
+        const bool ok = (e < 2 ? t.ok0 : t.ok1) && key >= row_lo[row] && key < row_hi[row];
+        if (!ok) sa[n][e] = -INFINITY;
+      }
+  }
   bool grow = false;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = n * 8 + 2 * c + (e & 1);
-      float s = (sa[n][e] + sb[n][e]) * (qs[n][e & 1] * (e < 2 ? t.ks0 : t.ks1));
-      const int key = t.t0 + g + (e < 2 ? 0 : 8);
-      if (row_slope) s = fmaf(row_slope[row], (float)(key - row_pos[row]), s);
-      bool ok = e < 2 ? t.ok0 : t.ok1;
-      if (masked) ok = ok && key >= row_lo[row] && key < row_hi[row];
-      sa[n][e] = ok ? s : -INFINITY;
-      grow = grow || sa[n][e] + (e < 2 ? lv0 : lv1) > st.m[n][e & 1];
-    }
-  }
+    for (int q = 0; q < 2; ++q) grow = grow || fmaxf(sa[n][q] + t.lv0, sa[n][q + 2] + t.lv1) > st.m[n][q];
   if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        float mx = fmaxf(sa[n][q] + lv0, sa[n][q + 2] + lv1);
+        float mx = fmaxf(sa[n][q] + t.lv0, sa[n][q + 2] + t.lv1);
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
         mx = fmaxf(mx, st.m[n][q]);
@@ -355,8 +363,12 @@ __device__ __forceinline__ void qa_step(const QaTile<D>& t, const uint32_t (&qf)
     for (int e = 0; e < 4; ++e) {
       const float pe = ex2_approx(sa[n][e] - st.m[n][e & 1]);
       st.l[n][e & 1] += pe;
-      // a masked key's scale may be anything
-      w[e] = sa[n][e] == -INFINITY ? 0.f : pe * (e < 2 ? v0 : v1);
+      w[e] = pe * (e < 2 ? v0 : v1);
+    }
+    if (masked) {  // a masked key's scale may be anything
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (sa[n][e] == -INFINITY) w[e] = 0.f;
     }
     const uint32_t h0 = qa_pack(w[0], w[1]), h1 = qa_pack(w[2], w[3]);
     pf[0][n][0] = qa_transpose(h0);
@@ -367,14 +379,23 @@ __device__ __forceinline__ void qa_step(const QaTile<D>& t, const uint32_t (&qf)
       pf[1][n][1] = qa_transpose(qa_pack(w[2] - f1.x, w[3] - f1.y));
     }
   }
+  uint32_t v[4][Q::VW];
 #pragma unroll
-  for (int w = 0; w < VW; ++w) {
+  for (int e = 0; e < 4; ++e) qa_lds<Q::VB>(stage + at.v[e & 1] + (e >> 1) * 8 * D, v[e]);
+  if (masked) {  // rows behind the keys may hold anything
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int w = 0; w < Q::VW; ++w) v[e][w] = t.okv[e] ? v[e][w] : 0u;
+  }
+#pragma unroll
+  for (int w = 0; w < Q::VW; ++w) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const uint32_t sel = hf ? 0x7362u : 0x5140u;
       uint32_t a0, a1, a2, a3;
-      qa_codes<INT8>(__byte_perm(t.v[0][w], t.v[1][w], sel), a0, a1);
-      qa_codes<INT8>(__byte_perm(t.v[2][w], t.v[3][w], sel), a2, a3);
+      qa_codes<INT8>(__byte_perm(v[0][w], v[1][w], sel), a0, a1);  // keys c, c + 4: P^T's rows 2c, 2c + 1
+      qa_codes<INT8>(__byte_perm(v[2][w], v[3][w], sel), a2, a3);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         qa_mma(st.acc[n][2 * w + hf], a0, a1, a2, a3, pf[0][n][0], pf[0][n][1]);
@@ -456,20 +477,53 @@ __device__ __forceinline__ int qa_cta_of(long long f, long long total, int grid)
   return (int)(((f + 1) * grid - 1) / total);
 }
 
+// Dynamic shared memory of the kernel: the warps' rings, or the warps' merge.
+template <int D, int NT, bool BS16>
+constexpr int qa_smem_bytes() {
+  using Q = QaRing<D>;
+  constexpr int ring = kQaWarps * (Q::kRing + (BS16 ? 0 : Q::kStages * Q::kMeta)), red = kQaWarps * 8 * NT * (D + 4) * 4;
+  return ring > red ? ring : red;
+}
+
 template <typename T, int D, int NT, bool INT8, bool BS16, int MINB>
-__global__ void __launch_bounds__(32 * kQaWarps, MINB) quant_attn_kernel(const QaParams p) {
+__global__ void __launch_bounds__(32 * kQaWarps, MINB)
+    quant_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                      const QaParams p) {
   constexpr bool SPLIT = sizeof(T) == 4;
   constexpr int ROWS = 8 * NT;
   constexpr int RED = D + 4;  // floats a row in the warps' merge: acc, m, l
   __shared__ int s_lo[ROWS], s_hi[ROWS], s_pos[ROWS];
   __shared__ float s_slope[4][ROWS];
   __shared__ long long s_sum[kQaWarps];
-  __shared__ int s_v;
+  __shared__ int s_v, s_abort;
+  __shared__ __align__(8) uint64_t s_bar[kQaWarps][QaRing<D>::kStages];
   __shared__ long long s_rem;
-  __shared__ __align__(16) float s_red[kQaWarps][ROWS][RED];
+  using Q = QaRing<D>;
+  extern __shared__ __align__(1024) unsigned char qa_smem[];
+  // the warps' rings; between units, the warps' merge ([warp][ROWS][RED] floats)
+  float(*s_red)[ROWS][RED] = reinterpret_cast<float(*)[ROWS][RED]>(qa_smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int HP = p.HP, KS = kQaWarps / HP;
   const int hp = warp % HP, kidx = warp / HP;
+  const uint32_t ring = smem_u32(qa_smem + warp * Q::kRing);
+  float* meta = reinterpret_cast<float*>(qa_smem + kQaWarps * Q::kRing + warp * Q::kStages * Q::kMeta);
+  const uint32_t bars = smem_u32(s_bar[warp]);
+  const int dim0 = qa_piece<D>(g) * (D / 8);  // of the lane's output dims
+  const QaLane<D> at(g, c);
+  const WaitCtx wctx{&s_abort, p.status, p.timeout_ns};
+  uint32_t phase = 0;                          // parity of each stage's next completion
+  int stage_in = 0, stage_out = 0;             // next stage to fill, to read
+  if constexpr (BS16) {
+    if (lane == 0) {
+      for (int i = 0; i < Q::kStages; ++i) mbar_init(bars + 8 * i, 1);
+      fence_mbar_init();
+    }
+    if (threadIdx.x == 0) {
+      s_abort = 0;
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+    }
+  }
   const int V = p.B * p.RT;
 
   // this CTA's range: total chunks, then the virtual sequence its first chunk falls in
@@ -565,22 +619,152 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB) quant_attn_kernel(const Q
     const int k0 = max((r.c0 + ch0) * kQaChunk, r.klo & ~(kQaTile - 1));
     const int k1 = min((long long)(r.c0 + ch1) * kQaChunk, (long long)r.khi);
     const int* bt = p.block_tables + (long long)b * p.bt_stride;
-    const long long head_off = hk * p.p_sh, head_sc = hk * p.sc_sh;
+    const long long head_sc = hk * p.sc_sh;
     const float* slope = p.alibi ? s_slope[hp] : nullptr;
-    const int step = kQaTile * KS;
-    int t0 = k0 + kidx * kQaTile;
-    QaTile<D> ta, tb;
-    if (t0 < k1) qa_load<D, BS16>(p, bt, head_off, head_sc, t0, k1, g, c, ta);
-    while (t0 < k1) {
-      if (t0 + step < k1) qa_load<D, BS16>(p, bt, head_off, head_sc, t0 + step, k1, g, c, tb);
-      qa_step<D, NT, SPLIT, INT8>(ta, qf, qs, s_lo, s_hi, slope, s_pos,
-                                  t0 < r.flo || t0 + kQaTile > r.fhi, g, c, st);
-      t0 += step;
-      if (t0 >= k1) break;
-      if (t0 + step < k1) qa_load<D, BS16>(p, bt, head_off, head_sc, t0 + step, k1, g, c, ta);
-      qa_step<D, NT, SPLIT, INT8>(tb, qf, qs, s_lo, s_hi, slope, s_pos,
-                                  t0 < r.flo || t0 + kQaTile > r.fhi, g, c, st);
-      t0 += step;
+    const int step = kQaTile * KS, ta = k0 + kidx * kQaTile;
+    const int tiles = ta < k1 ? (k1 - ta + step - 1) / step : 0;  // this warp's
+    if constexpr (BS16) {
+      // A tile lies in one block: lane i % 32 holds tile i's block and scales, for 32 tiles at a
+      // time, the next 32 being loaded while these are worked on.  A tile's K and V rows are one
+      // TMA box each, issued by lane 0; tiles without a block are skipped.
+      struct Batch {
+        int id;
+        float ks, vs, lv;
+        uint32_t there;  // which of the 32 have a block
+      };
+      auto batch = [&](int i0) {
+        Batch x{-1, 0.f, 0.f, 0.f, 0u};
+        const int i = i0 + lane;
+        if (i < tiles) {
+          const int got = __ldg(bt + (unsigned)(ta + i * step) / (unsigned)p.block_size);
+          if (got >= 0 && got < p.num_blocks) {
+            x.id = got;
+            x.ks = __ldg(p.k_scales + got * p.sc_sb + head_sc);
+            x.vs = __ldg(p.v_scales + got * p.sc_sb + head_sc);
+            x.lv = qa_log_scale(x.vs);
+          }
+        }
+        x.there = __ballot_sync(0xffffffffu, x.id >= 0);
+        return x;
+      };
+      Batch cur = batch(0), next = batch(32);
+      int base = 0;  // first tile of `cur`
+      int inflight = 0;
+      stage_in = stage_out;
+      auto issue = [&](int i) {
+        const bool far = i - base >= 32;
+        if (i >= tiles || !((far ? next.there : cur.there) >> (i & 31) & 1u)) return;
+        const int id = __shfl_sync(0xffffffffu, far ? next.id : cur.id, i & 31);
+        if (lane == 0) {
+          const unsigned t0 = ta + i * step;
+          const int row = p.bs_pow2 ? t0 & (p.block_size - 1) : t0 % (unsigned)p.block_size;
+          const uint32_t bar = bars + 8 * stage_in, dst = ring + stage_in * Q::kTileBytes;
+          mbar_arrive_expect_tx(bar, Q::kTileBytes);
+          tma_load_4d(dst, &tm_k, bar, 0, hk, row, id);
+          tma_load_4d(dst + Q::kHalf, &tm_v, bar, 0, hk, row, id);
+        }
+        stage_in = stage_in + 1 == Q::kStages ? 0 : stage_in + 1;
+        ++inflight;
+      };
+      fence_proxy_async_smem();  // the ring may have been the merge's buffer
+      __syncwarp();
+      int ahead = 0;             // tiles issued so far
+      for (; ahead < Q::kStages; ++ahead) issue(ahead);
+      bool ok = true;
+      for (int i = 0; i < tiles; ++i) {
+        if (cur.there >> (i & 31) & 1u) {
+          ok = __all_sync(0xffffffffu, mbar_wait(bars + 8 * stage_out, phase >> stage_out & 1u, wctx,
+                                                 kSiteQuantPaged));
+          if (!ok) break;
+          phase ^= 1u << stage_out;
+          --inflight;
+          const int t0 = ta + i * step;
+          QaRows rows;
+          rows.ks0 = rows.ks1 = __shfl_sync(0xffffffffu, cur.ks, i & 31);
+          rows.vs0 = rows.vs1 = __shfl_sync(0xffffffffu, cur.vs, i & 31);
+          rows.lv0 = rows.lv1 = __shfl_sync(0xffffffffu, cur.lv, i & 31);
+          rows.ok0 = t0 + qa_key(g) < k1;
+          rows.ok1 = t0 + qa_key(g) + 8 < k1;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) rows.okv[e] = t0 + c + 4 * e < k1;
+          qa_step<D, NT, SPLIT, INT8>(ring + stage_out * Q::kTileBytes, at, rows, t0, qf, qs, s_lo, s_hi,
+                                      slope, s_pos, t0 < r.flo || t0 + kQaTile > r.fhi, g, c, st);
+          stage_out = stage_out + 1 == Q::kStages ? 0 : stage_out + 1;
+          __syncwarp();  // every lane has read the stage
+          if (lane == 0) fence_proxy_async_smem();
+        }
+        // keep kStages tiles in flight: skipped tiles leave their stage to later ones
+        while (inflight < Q::kStages && ahead < tiles && ahead - base < 64) issue(ahead++);
+        if ((i & 31) == 31) {
+          base += 32;
+          cur = next;
+          next = batch(base + 32);
+          while (inflight < Q::kStages && ahead < tiles && ahead - base < 64) issue(ahead++);
+        }
+      }
+      if (!ok) {  // wait (bounded) for this warp's copies, then write nothing more
+        for (int k = 0; k < inflight; ++k) {
+          const int sk = (stage_out + k) % Q::kStages;
+          if (lane == 0) mbar_wait_drain(bars + 8 * sk, phase >> sk & 1u, p.status, p.timeout_ns);
+        }
+        __syncwarp();
+      }
+    } else {
+      // Any block size: every lane copies the pieces that it reads itself, with cp.async.
+      const unsigned char* kl = p.k_pool + hk * p.p_sh + Q::KB * c;
+      const unsigned char* vl = p.v_pool + hk * p.p_sh + Q::VB * qa_piece<D>(g);
+      auto locate = [&](int key, long long& off) {
+        off = 0;
+        if (key >= k1) return -1;
+        const unsigned slot = (unsigned)key / (unsigned)p.block_size;
+        const int got = __ldg(bt + slot);
+        if (got < 0 || got >= p.num_blocks) return -1;
+        off = (long long)got * p.p_sb + (long long)(key - (int)slot * p.block_size) * p.p_st;
+        return got;
+      };
+      auto issue = [&](int i) {
+        const uint32_t dst = ring + (i % Q::kStages) * Q::kTileBytes;
+        float* m = meta + (i % Q::kStages) * (Q::kMeta / 4);
+        const int t0 = ta + i * step;
+        int ok = 0;
+        long long off;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int id = locate(t0 + qa_key(g) + 8 * hf, off);
+          ok |= (id >= 0) << hf;
+#pragma unroll
+          for (int x = 0; x < Q::KP; ++x) qa_copy<Q::KB>(dst + at.k[x] + 8 * hf * D, kl + off + 64 * x, id >= 0);
+          m[32 * hf + lane] = id < 0 ? 0.f : __ldg(p.k_scales + id * p.sc_sb + head_sc);
+          m[64 + 32 * hf + lane] = id < 0 ? 0.f : __ldg(p.v_scales + id * p.sc_sb + head_sc);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool in = locate(t0 + c + 4 * e, off) >= 0;
+          ok |= in << (2 + e);
+          qa_copy<Q::VB>(dst + at.v[e & 1] + (e >> 1) * 8 * D, vl + off, in);
+        }
+        m[128 + lane] = __int_as_float(ok);
+      };
+      for (int i = 0; i < Q::kStages - 1; ++i) {
+        if (i < tiles) issue(i);
+        cp_async_commit();
+      }
+      for (int i = 0; i < tiles; ++i) {
+        if (i + Q::kStages - 1 < tiles) issue(i + Q::kStages - 1);  // into the stage used last
+        cp_async_commit();
+        cp_async_wait<Q::kStages - 1>();  // this lane's pieces of tile i have landed
+        const int t0 = ta + i * step;
+        const float* m = meta + (i % Q::kStages) * (Q::kMeta / 4);
+        const int ok = __float_as_int(m[128 + lane]);
+        QaRows rows{m[lane], m[32 + lane], m[64 + lane], m[96 + lane], 0.f, 0.f, (ok & 1) != 0, (ok & 2) != 0,
+                    {(ok & 4) != 0, (ok & 8) != 0, (ok & 16) != 0, (ok & 32) != 0}};
+        rows.lv0 = qa_log_scale(rows.vs0);
+        rows.lv1 = qa_log_scale(rows.vs1);
+        const bool masked = t0 < r.flo || t0 + kQaTile > r.fhi || !__all_sync(0xffffffffu, ok == 63);
+        qa_step<D, NT, SPLIT, INT8>(ring + (i % Q::kStages) * Q::kTileBytes, at, rows, t0, qf, qs, s_lo, s_hi,
+                                    slope, s_pos, masked, g, c, st);
+      }
+      cp_async_wait<0>();
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -590,6 +774,9 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB) quant_attn_kernel(const Q
         for (int off = 4; off < 32; off <<= 1)
           st.l[n][e] += __shfl_xor_sync(0xffffffffu, st.l[n][e], off);
 
+    if constexpr (BS16) {
+      if (__syncthreads_or(s_abort != 0)) break;  // a wait gave up: nothing more is written
+    }
     const bool whole = ch0 == 0 && ch1 == r.n;
     const long long slot = 2LL * blockIdx.x + (f == f_begin ? 0 : 1);
     if (KS == 1) {
@@ -603,14 +790,14 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB) quant_attn_kernel(const Q
             const int i = row / p.G, h = hk * p.G + row - i * p.G;
             const bool some = st.l[n][e] != 0.f && i < r.qlen;
             const float inv = 1.f / (st.l[n][e] * kQaPScale);
-            T* o = static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh + i * p.o_ss + g * (D / 8);
+            T* o = static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh + i * p.o_ss + dim0;
 #pragma unroll
             for (int d = 0; d < D / 16; ++d)
               qa_store2<T>(o + 2 * d, some ? st.acc[n][d][e] * inv : 0.f,
                            some ? st.acc[n][d][e + 2] * inv : 0.f);
           } else {
             const long long pr = (slot * HP + hp) * p.rows + tr;
-            float* o = p.o_part + pr * D + g * (D / 8);
+            float* o = p.o_part + pr * D + dim0;
 #pragma unroll
             for (int d = 0; d < D / 16; ++d)
               *reinterpret_cast<float2*>(o + 2 * d) = make_float2(st.acc[n][d][e], st.acc[n][d][e + 2]);
@@ -618,6 +805,7 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB) quant_attn_kernel(const Q
           }
         }
     } else {
+      __syncthreads();  // every warp is done with its ring
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -625,7 +813,7 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB) quant_attn_kernel(const Q
           float* row = s_red[warp][n * 8 + 2 * c + e];
 #pragma unroll
           for (int d = 0; d < D / 16; ++d)
-            *reinterpret_cast<float2*>(row + g * (D / 8) + 2 * d) =
+            *reinterpret_cast<float2*>(row + dim0 + 2 * d) =
                 make_float2(st.acc[n][d][e], st.acc[n][d][e + 2]);
           if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(st.m[n][e], st.l[n][e]);
         }

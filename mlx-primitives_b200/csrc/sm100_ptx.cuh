@@ -96,6 +96,18 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const W
   return mbar_wait_slow(bar, parity, w, site);
 }
 
+constexpr int kSiteDrain = 6;  // device-status site of drains, whichever kernel's
+
+// Wait without looking at the abort flag (used when draining after an abort).
+__device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity, int* status,
+                                                uint64_t timeout_ns) {
+  int dummy_flag = 0;
+  WaitCtx w{&dummy_flag, status, timeout_ns};
+  if (mbar_try_wait(bar, parity)) return true;
+  // mbar_wait_slow reads the flag through a volatile pointer; a private flag is never set.
+  return mbar_wait_slow(bar, parity, w, kSiteDrain);
+}
+
 // Bounded wait until *ctr >= target, a counter other CTAs raise with atomics (acquire load at
 // device scope, so their writes that precede the raise are visible afterwards).  Gives up like
 // mbar_wait: abort flag, time limit, poll cap; returns false then.
