@@ -20,7 +20,7 @@
 // in int8.
 //
 // One unit is (sequence, touched block, head, K or V), taken by WPU warps: they read the block's
-// new rows once, keep the rotated values in registers (64 a lane: 16 rows of 128 a warp), agree
+// new rows once, keep the rotated values in registers (32 a lane: 8 rows of 128 a warp), agree
 // on amax through shared memory and write the codes.  A block of more rows than the warps hold is
 // read a second time (from L2) instead.  Bound by HBM for prompts, by latency for single tokens.
 #pragma once
@@ -48,7 +48,8 @@ struct AppendParams {
   NormSpec q_norm, k_norm;
   const float *cosc, *sinc;
   long long n_pos;
-  int q_groups, k_groups;                 // units a token of q, and of each of k and v
+  int q_steps, q_groups;                  // row steps a unit of q, units a token
+  int k_groups;                           // units a token of each of k and v
   long long q_units, kv_units;            // row units (kv: 16/32-bit pools)
   int q_ctas;                             // 8-bit pools: CTAs [0, q_ctas) take the q units
   int touch;                              // 8-bit pools: blocks a sequence may touch
@@ -74,28 +75,39 @@ template <typename R, int U>
 __device__ __forceinline__ void append_q_unit(const AppendParams& p, unsigned u, int j, int g) {
   using T = typename R::T;
   const unsigned tok = u / (unsigned)p.q_groups;
-  const int h0 = (int)(u - tok * (unsigned)p.q_groups) * (R::RPW * U) + g;
+  const int first = (int)(u - tok * (unsigned)p.q_groups) * p.q_steps * R::RPW;
+  const int last = min(p.Hq, first + p.q_steps * R::RPW);
   const int b = (int)(tok / (unsigned)p.S), i = (int)(tok - (unsigned)b * (unsigned)p.S);
   const T* x = static_cast<const T*>(p.q) + b * p.q_s[0] + i * p.q_s[2];
+  T* y = static_cast<T*>(p.q_out) + b * p.qo_s[0] + i * p.qo_s[2];
+  // padding rows of a ragged batch are not read: their number is looked up first
+  const bool within = i < append_count(p, b);
   RowData<R> d[U];
+  auto load = [&](int h0) {
 #pragma unroll
-  for (int r = 0; r < U; ++r) {
-    const int h = h0 + r * R::RPW;
-    row_load<R>(x + h * p.q_s[1], p.half, j, h < p.Hq, d[r]);
-  }
+    for (int r = 0; r < U; ++r) {
+      const int h = h0 + r * R::RPW + g;
+      row_load<R>(x + h * p.q_s[1], p.half, j, within && h < last, d[r]);
+    }
+  };
+  load(first);
   RowCoef<R> k;
   coef_weights<R>(p.q_norm, p.half, j, k);
   const long long pos = (long long)__ldg(p.context_lens + b) + i;
-  const bool live = i < append_count(p, b) && pos >= 0 && pos < (long long)p.max_blocks * p.block_size;
+  const bool live = within && pos >= 0 && pos < (long long)p.max_blocks * p.block_size;
   coef_tables<R>(p.cosc, p.sinc, live ? pos : 0, p.half, j, k);
-  T* y = static_cast<T*>(p.q_out) + b * p.qo_s[0] + i * p.qo_s[2];
+  for (int h0 = first;;) {
 #pragma unroll
-  for (int r = 0; r < U; ++r) {
-    const int h = h0 + r * R::RPW;
-    float y1[R::NE], y2[R::NE];
-    row_norm_rope<R>(d[r], p.q_norm, p.cosc != nullptr, k, y1, y2);
-    if (!live) fill2<R::NE>(0.f, y1, y2);
-    if (h < p.Hq) row_store<R>(y + h * p.qo_s[1], p.half, j, y1, y2);
+    for (int r = 0; r < U; ++r) {
+      const int h = h0 + r * R::RPW + g;
+      float2 y1[R::NP], y2[R::NP];
+      row_norm_rope<R>(d[r], p.q_norm, p.cosc != nullptr, k, y1, y2);
+      if (!live) fill2<R::NP>(0.f, y1, y2);
+      if (h < last) row_store<R>(y + h * p.qo_s[1], p.half, j, y1, y2);
+    }
+    h0 += U * R::RPW;
+    if (h0 >= last) return;
+    load(h0);
   }
 }
 
@@ -136,13 +148,10 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 #pragma unroll
     for (int r = 0; r < U; ++r) {
       const int h = h0 + r * R::RPW;
-      float y1[R::NE], y2[R::NE];
+      float2 y1[R::NP], y2[R::NP];
       if (is_v) {
-#pragma unroll
-        for (int e = 0; e < R::NE; ++e) {
-          y1[e] = to_f<T>(d[r].x1[e]);
-          y2[e] = to_f<T>(d[r].x2[e]);
-        }
+        row_to_f<R>(d[r].x1, y1);
+        row_to_f<R>(d[r].x2, y2);
       } else {
         row_norm_rope<R>(d[r], p.k_norm, p.cosc != nullptr, k, y1, y2);
       }
@@ -188,9 +197,15 @@ __device__ __forceinline__ void store_codes(unsigned char* y, const float* x) {
     unsigned w[VEC / 4];
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i) {
-      w[i] = 0;
+      if constexpr (INT8) {
+        w[i] = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[i] |= to_code<INT8>(x[4 * i + e]) << (8 * e);
+        for (int e = 0; e < 4; ++e) w[i] |= to_code<INT8>(x[4 * i + e]) << (8 * e);
+      } else {
+        const unsigned lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i], x[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+        const unsigned hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2], x[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
+        w[i] = lo | hi << 16;
+      }
     }
     if constexpr (VEC == 8) *reinterpret_cast<uint2*>(y) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<unsigned*>(y) = w[0];
@@ -198,10 +213,10 @@ __device__ __forceinline__ void store_codes(unsigned char* y, const float* x) {
 }
 
 template <typename R>
-__host__ __device__ constexpr int append_steps() { return 64 / (2 * R::NE); }  // row steps a warp keeps
+__host__ __device__ constexpr int append_steps() { return 32 / (2 * R::NE); }  // row steps a warp keeps
 
 template <typename R, int U, bool INT8>
-__global__ void __launch_bounds__(256) append_quant_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(256, 2) append_quant_kernel(const AppendParams p) {
   using T = typename R::T;
   constexpr int STEPS = append_steps<R>();
   constexpr int ROWS = STEPS * R::RPW;    // rows a warp keeps
@@ -246,7 +261,7 @@ __global__ void __launch_bounds__(256) append_quant_kernel(const AppendParams p)
     const int first = r0 / stride, n = on ? (r1 - 1) / stride - first + 1 : 0;
     RowCoef<R> kw;
     if (on && !is_v) coef_weights<R>(p.k_norm, p.half, j, kw);
-    float y1[STEPS][R::NE], y2[STEPS][R::NE];
+    float2 y1[STEPS][R::NP], y2[STEPS][R::NP];
     float s_new = 1.f;
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
@@ -268,16 +283,13 @@ __global__ void __launch_bounds__(256) append_quant_kernel(const AppendParams p)
             const int r = row0 + i * R::RPW;
             const bool live = r >= r0 && r < r1;
             if (is_v) {
-#pragma unroll
-              for (int e = 0; e < R::NE; ++e) {
-                y1[i][e] = to_f<T>(d[i].x1[e]);
-                y2[i][e] = to_f<T>(d[i].x2[e]);
-              }
+              row_to_f<R>(d[i].x1, y1[i]);
+              row_to_f<R>(d[i].x2, y2[i]);
             } else if (__any_sync(0xffffffffu, live)) {
               coef_tables<R>(p.cosc, p.sinc, live ? base + r : 0, p.half, j, kw);
               row_norm_rope<R>(d[i], p.k_norm, p.cosc != nullptr, kw, y1[i], y2[i]);
             } else {
-              fill2<R::NE>(0.f, y1[i], y2[i]);
+              fill2<R::NP>(0.f, y1[i], y2[i]);
             }
           }
         }
@@ -286,12 +298,21 @@ __global__ void __launch_bounds__(256) append_quant_kernel(const AppendParams p)
           const int r = row0 + i * R::RPW;
           const bool live = r >= r0 && r < r1;
           if (pass == 0) {
+            // the largest first; where it is not finite, the finite ones one by one (the maximum
+            // passes NaN over, which the clamp's code keeps)
+            float big = 0.f;
 #pragma unroll
-            for (int e = 0; e < R::NE; ++e) {
-              const float a = fabsf(y1[i][e]), c = fabsf(y2[i][e]);
-              if (live && a <= 3.402823466e38f) amax = fmaxf(amax, a);
-              if (live && c <= 3.402823466e38f) amax = fmaxf(amax, c);
+            for (int e = 0; e < R::NP; ++e)
+              big = fmaxf(fmaxf(big, fmaxf(fabsf(y1[i][e].x), fabsf(y1[i][e].y))),
+                          fmaxf(fabsf(y2[i][e].x), fabsf(y2[i][e].y)));
+            if (big > 3.402823466e38f) {
+              big = 0.f;
+#pragma unroll
+              for (int e = 0; e < R::NP; ++e)
+                for (const float a : {y1[i][e].x, y1[i][e].y, y2[i][e].x, y2[i][e].y})
+                  if (fabsf(a) <= 3.402823466e38f) big = fmaxf(big, fabsf(a));
             }
+            if (live) amax = fmaxf(amax, big);
           } else if (live) {
 #pragma unroll
             for (int c = 0; c < R::NC; ++c) {
@@ -300,7 +321,9 @@ __global__ void __launch_bounds__(256) append_quant_kernel(const AppendParams p)
               float a[R::VEC], e2[R::VEC];
 #pragma unroll
               for (int e = 0; e < R::VEC; ++e) {
-                const float f1 = y1[i][c * R::VEC + e], f2 = y2[i][c * R::VEC + e];
+                const int x = c * R::VEC + e;
+                const float f1 = x & 1 ? y1[i][x / 2].y : y1[i][x / 2].x;
+                const float f2 = x & 1 ? y2[i][x / 2].y : y2[i][x / 2].x;
                 a[e] = divide ? __fdiv_rn(f1, s_new) : f1 * inv;
                 e2[e] = divide ? __fdiv_rn(f2, s_new) : f2 * inv;
               }

@@ -14,7 +14,6 @@
 namespace mlxp {
 namespace {
 
-constexpr int kBwdCtasPerSm = 2;   // of 256 threads: the backward's registers allow two
 constexpr int kMaxGridSms = 256;   // workspace bound; devices have fewer SMs
 
 int check_dtype(int64_t dt, const char* what) {
@@ -65,10 +64,13 @@ int with_row_shape(int64_t dtype, int half, bool wide, F&& f) {
   return with_row_shape_t<__half>(half, wide, f);
 }
 
-// Row steps of a unit.  Four 16-byte steps put 4 KB a warp in flight in the forward; the backward
-// loads twice as much a row.
+// Row steps loaded at a time and the CTAs of 256 threads an SM holds (the registers' limit).
+// Measured on 2 x 16384 x 64 rows of 128 bf16, units of U steps: forward 199 us at (2, 3), 220 at
+// (4, 2), 266 at (2, 2); backward 335 at (2, 2), 443 at (2, 1), 362 at (4, 1).  Units of whole
+// tokens, at (2, 3) and (2, 2): 184 us (5.8 TB/s) and 280 us (5.8 TB/s).
+constexpr int kFwdCtas = 3, kBwdCtas = 2;
 template <typename R>
-constexpr int fwd_steps() { return R::kWide ? 4 : 2; }
+constexpr int fwd_steps() { return 2; }
 template <typename R>
 constexpr int bwd_steps() { return R::kWide ? 2 : 1; }
 
@@ -157,10 +159,18 @@ NormRopeParams norm_rope_params(const mlxp_qk_norm_rope_args* a, bool bwd, bool&
   return p;
 }
 
-// Units of both tensors for `heads` heads a unit.
-void count_units(NormRopeParams& p, int64_t B, int heads) {
+// Row steps a unit (one warp's work at a time) takes of a token's `all`: all of them where the
+// tokens alone fill the SMs' warps, else the kernel's U.
+int unit_steps(long long tokens, int all, int U, int sms) {
+  return tokens >= 24LL * sms ? std::max(all, 1) : U;
+}
+
+// Units of both tensors for rpw rows a step.
+void count_units(NormRopeParams& p, int64_t B, int rpw, int U, int sms) {
   for (NormRopeTensor& t : p.t) {
-    t.groups = std::max(1, (t.H + heads - 1) / heads);
+    const int all = (t.H + rpw - 1) / rpw;
+    t.steps = unit_steps(B * t.S, all, U, sms);
+    t.groups = std::max(1, (all + t.steps - 1) / t.steps);
     t.units = t.H ? B * t.S * (long long)t.groups : 0;
   }
 }
@@ -182,19 +192,19 @@ int mlxp_qk_norm_rope(const mlxp_qk_norm_rope_args* a) {
   return with_row_shape(a->dtype, p.half, wide, [&](auto shape) {
     using R = decltype(shape);
     constexpr int U = fwd_steps<R>();
-    count_units(p, a->B, R::RPW * U);
+    count_units(p, a->B, R::RPW, U, sms);
     const long long units = p.t[0].units + p.t[1].units;
     // few units: one warp a block, so that they spread over the SMs
     const int warps = units >= 8LL * sms ? 8 : 1;
     const long long grid = std::min<long long>((units + warps - 1) / warps, 64LL * sms);
-    norm_rope_kernel<R, U><<<(unsigned)grid, 32 * warps, 0, (cudaStream_t)a->stream>>>(p);
+    norm_rope_kernel<R, U, kFwdCtas><<<(unsigned)grid, 32 * warps, 0, (cudaStream_t)a->stream>>>(p);
     return launched("qk_norm_rope launch");
   });
 }
 
 size_t mlxp_qk_norm_rope_bwd_workspace_size(int64_t D) {
   if (D < 2 || D > 256) return 0;
-  return (size_t)kMaxGridSms * kBwdCtasPerSm * 2 * D * sizeof(float);
+  return (size_t)kMaxGridSms * kBwdCtas * 2 * D * sizeof(float);
 }
 
 int mlxp_qk_norm_rope_bwd(const mlxp_qk_norm_rope_args* a) {
@@ -214,14 +224,14 @@ int mlxp_qk_norm_rope_bwd(const mlxp_qk_norm_rope_args* a) {
   return with_row_shape(a->dtype, p.half, wide, [&](auto shape) {
     using R = decltype(shape);
     constexpr int U = bwd_steps<R>();
-    count_units(p, a->B, R::RPW * U);
+    count_units(p, a->B, R::RPW, U, sms);
     const long long most = std::max(p.t[0].units, p.t[1].units);
     const long long grid =
-        std::max<long long>(1, std::min<long long>((most + 7) / 8, (long long)kBwdCtasPerSm * sms));
+        std::max<long long>(1, std::min<long long>((most + 7) / 8, (long long)kBwdCtas * sms));
     float* part = static_cast<float*>(a->workspace);
     p.t[0].dw_part = a->dq_weight ? part : nullptr;
     p.t[1].dw_part = a->dk_weight ? part + grid * a->D : nullptr;
-    norm_rope_bwd_kernel<R, U><<<(unsigned)grid, 256, 8 * a->D * sizeof(float), s>>>(p);
+    norm_rope_bwd_kernel<R, U, kBwdCtas><<<(unsigned)grid, 256, 8 * a->D * sizeof(float), s>>>(p);
     if (int rc = launched("qk_norm_rope backward launch")) return rc;
     if (!dw) return (int)MLXP_OK;
     NormRopeDw d{{p.t[0].dw_part, p.t[1].dw_part},
@@ -326,7 +336,9 @@ int mlxp_paged_append(const mlxp_paged_append_args* a) {
     constexpr int U = bwd_steps<R>();
     const int heads = R::RPW * U;
     const long long tokens = a->B * a->S;
-    p.q_groups = std::max(1, (p.Hq + heads - 1) / heads);
+    const int all = (p.Hq + R::RPW - 1) / R::RPW;
+    p.q_steps = unit_steps(tokens, all, U, sms);
+    p.q_groups = std::max(1, (all + p.q_steps - 1) / p.q_steps);
     p.k_groups = (p.Hk + heads - 1) / heads;
     p.q_units = p.Hq ? tokens * p.q_groups : 0;
     p.kv_units = tokens * p.k_groups;
