@@ -199,9 +199,13 @@ def address(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def raw_stream(device: torch.device) -> int:
-    """Handle of the device's current stream, without building a Stream object."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+# Handle of a device index's current stream, without building a Stream object.
+raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def plain(t: torch.Tensor, index: int, dtype: torch.dtype) -> bool:
+    """Whether a kernel can read t as it is: of this type, on this device, contiguous."""
+    return t.dtype is dtype and t.get_device() == index and t.is_contiguous()
 
 
 class _NoSwitch:
@@ -215,6 +219,6 @@ class _NoSwitch:
 _NO_SWITCH = _NoSwitch()
 
 
-def on_device(device: torch.device):
-    """Context in which `device` is the current device; free of cost where it already is."""
-    return _NO_SWITCH if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def on_device(index: int):
+    """Context in which device `index` is current; free of cost where it already is."""
+    return _NO_SWITCH if torch._C._cuda_getDevice() == index else torch.cuda.device(index)

@@ -23,6 +23,8 @@ _ARGS = _lib.ArgStruct(49, doubles=(47,))
 
 def _overlaps(t: torch.Tensor) -> bool:
     """Whether two elements of a strided tensor may share memory (sufficient for a view of rows)."""
+    if t.is_contiguous():
+        return False
     span = 1
     for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
         if stride < span:
@@ -33,36 +35,39 @@ def _overlaps(t: torch.Tensor) -> bool:
 
 def check_pools(k_pool, v_pool, k_scales, v_scales):
     """Checks that both cache operators make of the pools; returns the cache's dtype code."""
-    if k_pool.ndim != 4 or k_pool.shape != v_pool.shape:
+    shape, dtype, strides = k_pool.shape, k_pool.dtype, k_pool.stride()
+    if len(shape) != 4 or v_pool.shape != shape:
         raise ValueError("k_pool and v_pool must both be (num_blocks, block_size, heads, head_dim)"
                          f", got {tuple(k_pool.shape)} and {tuple(v_pool.shape)}")
-    if k_pool.dtype != v_pool.dtype:
+    if v_pool.dtype is not dtype:
         raise ValueError(f"k_pool and v_pool must share a dtype, got {k_pool.dtype} and {v_pool.dtype}")
-    if k_pool.stride() != v_pool.stride() or k_pool.stride(3) != 1:
+    if v_pool.stride() != strides or strides[3] != 1:
         raise ValueError("k_pool and v_pool must have the same strides, and unit head_dim stride, "
                          f"got {k_pool.stride()} and {v_pool.stride()}")
-    code = _lib.CACHE_DTYPE_CODES.get(k_pool.dtype)
+    code = _lib.CACHE_DTYPE_CODES.get(dtype)
     if code is None:
         if k_scales is not None or v_scales is not None:
             raise ValueError(f"scales go with float8_e4m3fn or int8 pools, got {k_pool.dtype}")
-        return _lib.DTYPE_CODES.get(k_pool.dtype)
-    want = (k_pool.shape[0], k_pool.shape[2])
+        return _lib.DTYPE_CODES.get(dtype)
+    dev = k_pool.get_device()
     for name, s in (("k_scales", k_scales), ("v_scales", v_scales)):
-        if s is None or s.dtype != torch.float32 or tuple(s.shape) != want or s.device != k_pool.device:
-            raise ValueError(f"{name} must be a float32 tensor (num_blocks, heads) = {want} beside "
-                             f"the pools, got {None if s is None else (s.dtype, tuple(s.shape), s.device)}")
+        if (s is None or s.dtype is not torch.float32 or s.shape != (shape[0], shape[2])
+                or s.get_device() != dev):
+            raise ValueError(f"{name} must be a float32 tensor (num_blocks, heads) = "
+                             f"{(shape[0], shape[2])} beside the pools, got "
+                             f"{None if s is None else (s.dtype, tuple(s.shape), s.device)}")
     if k_scales.stride() != v_scales.stride():
         raise ValueError("k_scales and v_scales must have the same strides")
     return code
 
 
-def device_ints(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
-    """Tables and lengths as the kernels read them: int32 on the device, unit inner stride."""
-    if t.dtype != torch.int32 or t.device != dev:
+def device_ints(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    """Tables and lengths as the kernels read them: int32 beside `like`, unit inner stride."""
+    if t.dtype is not torch.int32 or t.get_device() != like.get_device():
         if t.is_floating_point():
             raise ValueError(f"block tables and lengths must be integers, got {t.dtype}")
-        t = t.to(dev, torch.int32)
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+        t = t.to(like.device, torch.int32)
+    return t if t.is_contiguous() or t.stride(-1) == 1 else t.contiguous()
 
 
 def paged_append(
@@ -101,81 +106,119 @@ def paged_append(
     it to.  A block that receives tokens must belong to one sequence (full blocks may be shared):
     the order of two writers of a block is not defined.  Not differentiable.
     """
-    if k.ndim != 4 or k.shape != v.shape:
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape:
         raise ValueError("k and v must both be (batch, seq, kv_heads, head_dim), got "
                          f"{tuple(k.shape)} and {tuple(v.shape)}")
-    B, S, Hk, D = k.shape
+    B, S, Hk, D = shape
+    codes = _lib.DTYPE_CODES
     dtype = k.dtype
-    code = _lib.DTYPE_CODES.get(dtype)
-    if code is None or v.dtype != dtype:
+    code = codes.get(dtype)
+    if code is None or v.dtype is not dtype:
         raise ValueError(f"k and v must share a dtype of float32, bfloat16, float16, got {dtype}, {v.dtype}")
     cache_code = check_pools(k_pool, v_pool, k_scales, v_scales)
-    quant = k_pool.dtype in _lib.CACHE_DTYPE_CODES
-    if not quant and k_pool.dtype != dtype:
+    quant = k_scales is not None
+    if not quant and k_pool.dtype is not dtype:
         raise ValueError(f"the pools' dtype ({k_pool.dtype}) must be k's ({dtype}) or an 8-bit one")
     num_blocks, block_size, Hp, Dp = k_pool.shape
     if Hp != Hk or Dp != D:
         raise ValueError(f"pools of (heads, head_dim) = {(Hp, Dp)} cannot take k of {(Hk, D)}")
     if D % 2 or D < 2:
         raise ValueError(f"head_dim must be even, got {D}")
-    dev = k.device
-    if dev.type != "cuda" or k_pool.device != dev or v_pool.device != dev or v.device != dev:
+    dev = k.get_device()
+    if dev < 0 or k_pool.get_device() != dev or v_pool.get_device() != dev or v.get_device() != dev:
         raise ValueError("k, v and the pools must be on one CUDA device (appending is in place)")
     if _overlaps(k_pool) or (quant and _overlaps(k_scales)):
         raise ValueError("the pools and scales must not overlap themselves (expanded views)")
-    if block_tables.ndim != 2 or block_tables.shape[0] != B:
+    bt_shape = block_tables.shape
+    if len(bt_shape) != 2 or bt_shape[0] != B:
         raise ValueError(f"block_tables must be (batch, max_blocks), got {tuple(block_tables.shape)}")
-    for name, t in (("context_lens", context_lens), ("new_lens", new_lens)):
-        if t is not None and tuple(t.shape) != (B,):
-            raise ValueError(f"{name} must be (batch,) = ({B},), got {tuple(t.shape)}")
-    Hq, q_strides = 0, (0, 0, 0)
+    max_blocks = bt_shape[1]
+    if context_lens.shape != (B,) or (new_lens is not None and new_lens.shape != (B,)):
+        raise ValueError(f"context_lens and new_lens must be (batch,) = ({B},), got "
+                         f"{tuple(context_lens.shape)} and {None if new_lens is None else tuple(new_lens.shape)}")
+    grad = torch.is_grad_enabled()
+    if grad and (k.requires_grad or v.requires_grad):
+        _no_gradients()
+    q_ptr = qo_ptr = Hq = 0
+    qs = qo = (0, 0, 0, 1)
+    q_out = None
     if q is not None:
-        if q.ndim != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != D or q.dtype != dtype or q.device != dev:
+        q_shape = q.shape
+        if (len(q_shape) != 4 or q_shape[0] != B or q_shape[1] != S or q_shape[3] != D
+                or q.dtype is not dtype or q.get_device() != dev):
             raise ValueError(f"q must be ({B}, {S}, heads, {D}) {dtype} beside k, got {tuple(q.shape)} {q.dtype}")
-        Hq = q.shape[2]
+        if grad and q.requires_grad:
+            _no_gradients()
+        Hq = q_shape[2]
+        qs = q.stride()
+        if qs[3] != 1:
+            q = q.contiguous()
+            qs = q.stride()
+        q_out = torch.empty_like(q)
+        q_ptr, qo_ptr, qo = q.data_ptr(), q_out.data_ptr(), q_out.stride()
     elif q_weight is not None:
         raise ValueError("q_weight needs q")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (tuple(w.shape) != (D,) or w.dtype not in _lib.DTYPE_CODES):
-            raise ValueError(f"{name} must be ({D},) of a supported dtype, got {tuple(w.shape)} {w.dtype}")
+    qw_ptr = kw_ptr = qw_code = kw_code = 0
+    if q_weight is not None:
+        q_weight = _weight("q_weight", q_weight, D, k, grad)
+        qw_ptr, qw_code = q_weight.data_ptr(), codes[q_weight.dtype]
+    if k_weight is not None:
+        k_weight = _weight("k_weight", k_weight, D, k, grad)
+        kw_ptr, kw_code = k_weight.data_ptr(), codes[k_weight.dtype]
     if (cos_cache is None) != (sin_cache is None):
         raise ValueError("cos_cache and sin_cache must be given together")
-    max_blocks = block_tables.shape[1]
-    n_pos = 0
+    n_pos = cos_ptr = sin_ptr = 0
     if cos_cache is not None:
-        if cos_cache.shape != sin_cache.shape or cos_cache.ndim != 2 or cos_cache.shape[1] != D // 2:
+        c_shape = cos_cache.shape
+        if len(c_shape) != 2 or c_shape[1] * 2 != D or sin_cache.shape != c_shape:
             raise ValueError("cos/sin caches must both be (max_seq, head_dim // 2)")
-        n_pos = cos_cache.shape[0]
+        n_pos = c_shape[0]
         if n_pos < max_blocks * block_size:
             raise ValueError(f"cos/sin caches of {n_pos} positions do not cover the block tables' "
                              f"{max_blocks * block_size}")
-        cos_cache, sin_cache = (c if c.dtype == torch.float32 and c.device == dev and c.is_contiguous()
-                                else c.to(dev, torch.float32).contiguous() for c in (cos_cache, sin_cache))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in
-                                       (k, v, q, q_weight, k_weight)):
-        raise NotImplementedError("paged_append is not differentiable: call it under torch.no_grad()")
-    bt, ctx = device_ints(block_tables, dev), device_ints(context_lens, dev)
-    new = None if new_lens is None else device_ints(new_lens, dev)
-    k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (k, v))
-    q_weight, k_weight = (w if w is None or (w.device == dev and w.is_contiguous())
-                          else w.to(dev).contiguous() for w in (q_weight, k_weight))
-    q_out, qo_strides = None, (0, 0, 0)
-    if q is not None:
-        q = q if q.stride(3) == 1 else q.contiguous()
-        q_out = torch.empty_like(q)
-        q_strides, qo_strides = _lib.seq_strides(q), _lib.seq_strides(q_out)
-    a = _lib.address
-    codes = _lib.DTYPE_CODES
+        if not _lib.plain(cos_cache, dev, torch.float32):
+            cos_cache = cos_cache.to(k.device, torch.float32).contiguous()
+        if not _lib.plain(sin_cache, dev, torch.float32):
+            sin_cache = sin_cache.to(k.device, torch.float32).contiguous()
+        cos_ptr, sin_ptr = cos_cache.data_ptr(), sin_cache.data_ptr()
+    bt, ctx = device_ints(block_tables, k), device_ints(context_lens, k)
+    new_ptr = 0
+    if new_lens is not None:
+        new_lens = device_ints(new_lens, k)
+        new_ptr = new_lens.data_ptr()
+    ks, vs = k.stride(), v.stride()
+    if ks[3] != 1:
+        k = k.contiguous()
+        ks = k.stride()
+    if vs[3] != 1:
+        v = v.contiguous()
+        vs = v.stride()
+    ps = k_pool.stride()
+    ksc_ptr = vsc_ptr = 0
+    sc = (0, 0)
+    if quant:
+        ksc_ptr, vsc_ptr, sc = k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride()
     with _lib.on_device(dev):
         rc = _lib.lib().mlxp_paged_append(_ARGS.pack(
-            k.data_ptr(), v.data_ptr(), a(q), a(q_out), k_pool.data_ptr(), v_pool.data_ptr(),
-            a(k_scales), a(v_scales), bt.data_ptr(), ctx.data_ptr(), a(new), a(q_weight),
-            a(k_weight), a(cos_cache), a(sin_cache), code, cache_code,
-            0 if q_weight is None else codes[q_weight.dtype],
-            0 if k_weight is None else codes[k_weight.dtype],
+            k.data_ptr(), v.data_ptr(), q_ptr, qo_ptr, k_pool.data_ptr(), v_pool.data_ptr(),
+            ksc_ptr, vsc_ptr, bt.data_ptr(), ctx.data_ptr(), new_ptr, qw_ptr, kw_ptr, cos_ptr,
+            sin_ptr, code, cache_code, qw_code, kw_code,
             B, S, Hq, Hk, D, num_blocks, block_size, max_blocks, bt.stride(0), n_pos,
-            *_lib.seq_strides(k), *_lib.seq_strides(v), *q_strides, *qo_strides,
-            *k_pool.stride()[:3], *(k_scales.stride() if quant else (0, 0)),
-            eps, _lib.raw_stream(dev)))
-    _lib.check(rc, "mlxp_paged_append")
+            ks[0], ks[2], ks[1], vs[0], vs[2], vs[1], qs[0], qs[2], qs[1], qo[0], qo[2], qo[1],
+            ps[0], ps[1], ps[2], sc[0], sc[1], eps, _lib.raw_stream(dev)))
+    if rc:
+        _lib.check(rc, "mlxp_paged_append")
     return q_out
+
+
+def _no_gradients():
+    raise NotImplementedError("paged_append is not differentiable: call it under torch.no_grad()")
+
+
+def _weight(name, w, D, k, grad):
+    if w.shape != (D,) or w.dtype not in _lib.DTYPE_CODES:
+        raise ValueError(f"{name} must be ({D},) of a supported dtype, got {tuple(w.shape)} {w.dtype}")
+    if grad and w.requires_grad:
+        _no_gradients()
+    return w if _lib.plain(w, k.get_device(), w.dtype) else w.to(k.device).contiguous()

@@ -13,7 +13,6 @@ row, as the reference does.)
 
 from __future__ import annotations
 
-import math
 from typing import Optional
 
 import torch
@@ -31,8 +30,7 @@ _HEAD_DIMS = (32, 64, 128)
 def _rows16(t: torch.Tensor) -> bool:
     es = t.element_size()
     s = t.stride()
-    return (s[3] == 1 and t.data_ptr() % 16 == 0 and s[0] * es % 16 == 0 and s[1] * es % 16 == 0
-            and s[2] * es % 16 == 0)
+    return s[3] == 1 and not (t.data_ptr() | s[0] * es | s[1] * es | s[2] * es) & 15
 
 
 def quantized_paged_attention(
@@ -61,13 +59,14 @@ def quantized_paged_attention(
     ALiBi adds slope[h] * (key position - query position).  Returns q's shape and dtype.  Not
     differentiable.
     """
-    if q.ndim != 4:
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError(f"q must be (batch, seq_q, num_heads, head_dim), got {tuple(q.shape)}")
     cache_code = check_pools(k_pool, v_pool, k_scales, v_scales)
-    if k_pool.dtype not in _lib.CACHE_DTYPE_CODES:
+    if k_scales is None:
         raise ValueError(f"the pools must be float8_e4m3fn or int8, got {k_pool.dtype}; "
                          "paged_attention reads other types")
-    B, Sq, H, D = q.shape
+    B, Sq, H, D = shape
     num_blocks, block_size, Hk, Dk = k_pool.shape
     if Dk != D:
         raise ValueError(f"pool head_dim ({Dk}) must equal q's head_dim ({D})")
@@ -78,52 +77,55 @@ def quantized_paged_attention(
     code = _lib.DTYPE_CODES.get(q.dtype)
     if code is None:
         raise ValueError(f"unsupported dtype {q.dtype}; expected float32, bfloat16 or float16")
-    if block_tables.ndim != 2 or block_tables.shape[0] != B:
+    bt_shape = block_tables.shape
+    if len(bt_shape) != 2 or bt_shape[0] != B:
         raise ValueError(f"block_tables must be (batch, max_blocks), got {tuple(block_tables.shape)}")
-    for name, t in (("context_lens", context_lens), ("query_lens", query_lens)):
-        if t is not None and tuple(t.shape) != (B,):
-            raise ValueError(f"{name} must be (batch,) = ({B},), got {tuple(t.shape)}")
-    if alibi_slopes is not None and tuple(alibi_slopes.shape) != (H,):
+    if context_lens.shape != (B,):
+        raise ValueError(f"context_lens must be (batch,) = ({B},), got {tuple(context_lens.shape)}")
+    if query_lens is not None and query_lens.shape != (B,):
+        raise ValueError(f"query_lens must be (batch,) = ({B},), got {tuple(query_lens.shape)}")
+    if alibi_slopes is not None and alibi_slopes.shape != (H,):
         raise ValueError(f"alibi_slopes must be (num_heads,) = ({H},), got {tuple(alibi_slopes.shape)}")
     if window_size is not None and window_size < 0:
         raise ValueError(f"window_size must be >= 0, got {window_size}")
-    if torch.is_grad_enabled() and q.requires_grad:
+    if q.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("quantized_paged_attention is not differentiable: call it under "
                                   "torch.no_grad()")
-    host = q.device.type == "cpu"
+    dev = q.get_device()
+    host = dev < 0
     if host:
         if not torch.cuda.is_available():
             raise RuntimeError("attention requires a CUDA device (there is no CPU fallback)")
-        dev = torch.device("cuda", torch.cuda.current_device())
+        dev = torch.cuda.current_device()
         q, k_pool, v_pool, k_scales, v_scales = (
             t.to(dev) for t in (q, k_pool, v_pool, k_scales, v_scales))
-    else:
-        dev = q.device
-    if k_pool.device != dev or v_pool.device != dev:
+    elif k_pool.get_device() != dev or v_pool.get_device() != dev:
         raise ValueError("q, k_pool and v_pool must be on the same device")
     if not _rows16(q):
-        q = q.contiguous() if q.data_ptr() % 16 == 0 or not q.is_contiguous() else q.clone()
-    bt, ctx = device_ints(block_tables, dev), device_ints(context_lens, dev)
-    lens = None if query_lens is None else device_ints(query_lens, dev)
-    slopes = None
+        q = q.clone(memory_format=torch.contiguous_format)
+    bt, ctx = device_ints(block_tables, q), device_ints(context_lens, q)
+    lens_ptr = slopes_ptr = 0
+    if query_lens is not None:
+        query_lens = device_ints(query_lens, q)
+        lens_ptr = query_lens.data_ptr()
     if alibi_slopes is not None:
-        slopes = alibi_slopes.to(dev, torch.float32).contiguous()
-    out = torch.empty((B, Sq, H, D), dtype=q.dtype, device=dev)
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
+        alibi_slopes = alibi_slopes.to(q.device, torch.float32).contiguous()
+        slopes_ptr = alibi_slopes.data_ptr()
+    out = torch.empty_like(q)
+    qs, os, ps, sc = q.stride(), out.stride(), k_pool.stride(), k_scales.stride()
     L = _lib.lib()
-    a = _lib.address
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
         fields = (q.data_ptr(), out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
-                  k_scales.data_ptr(), v_scales.data_ptr(), bt.data_ptr(), ctx.data_ptr(), a(lens),
-                  a(slopes), code, cache_code, B, Sq, H, Hk, D, num_blocks, block_size,
-                  bt.shape[1], bt.stride(0), 1 if causal else 0,
+                  k_scales.data_ptr(), v_scales.data_ptr(), bt.data_ptr(), ctx.data_ptr(), lens_ptr,
+                  slopes_ptr, code, cache_code, B, Sq, H, Hk, D, num_blocks, block_size,
+                  bt_shape[1], bt.stride(0), 1 if causal else 0,
                   -1 if window_size is None else int(window_size),
-                  *_lib.seq_strides(q), *_lib.seq_strides(out), *k_pool.stride()[:3],
-                  *k_scales.stride(), scale)
+                  qs[0], qs[2], qs[1], os[0], os[2], os[1], ps[0], ps[1], ps[2], sc[0], sc[1],
+                  D ** -0.5 if scale is None else scale)
         ws_bytes = L.mlxp_quant_paged_attn_workspace_size(_ARGS.pack(*fields, 0, 0, stream))
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        rc = L.mlxp_quant_paged_attn(_ARGS.pack(*fields, a(ws), ws_bytes, stream))
-    _lib.check(rc, "mlxp_quant_paged_attn")
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        rc = L.mlxp_quant_paged_attn(_ARGS.pack(*fields, ws.data_ptr(), ws_bytes, stream))
+    if rc:
+        _lib.check(rc, "mlxp_quant_paged_attn")
     return out.cpu() if host else out
