@@ -20,7 +20,8 @@ CSRC = Path(__file__).resolve().parent
 PKG_ROOT = CSRC.parent
 INCLUDE = PKG_ROOT.parent / "include"
 OUT = PKG_ROOT / "mlx_primitives" / "libmlxp_attn.so"
-SOURCES = [CSRC / "mlxp_attn.cu", CSRC / "mlxp_cache.cu", CSRC / "mlxp_quant.cu"]
+SOURCES = [CSRC / "mlxp_attn.cu", CSRC / "mlxp_cache.cu", CSRC / "mlxp_quant.cu",
+           CSRC / "mlxp_quant_rows.cu"]
 DEPS = SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [INCLUDE / "mlxp_attn.h"]
 OBJ = CSRC / "_build"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -9,12 +9,22 @@
 
 #include "../../include/mlxp_attn.h"
 #include "host_common.h"
-#include "quant_attn.cuh"
+#include "quant_attn_rows.cuh"
 
 namespace mlxp {
+
+MLXP_INTERNAL int qa_rows_launch(int64_t dtype, int64_t D, bool int8, const QaParams& p, unsigned grid,
+                                 cudaStream_t s);  // mlxp_quant_rows.cu
+
 namespace {
 
+#ifndef QR_FROM
+#define QR_FROM 64
+#endif
+constexpr int kRowsFrom = QR_FROM;
+
 struct QaPlan {
+  bool many;         // the many-row kernel
   int nt;            // 8-row query tiles a warp
   int per_sm;        // CTAs an SM holds
   long long grid;
@@ -74,6 +84,16 @@ QaPlan qa_plan(const mlxp_quant_paged_attn_args* a, int sms, QaParams& p) {
   p.G = (int)(a->H / a->kv_heads);
   p.Sq = (int)a->Sq;
   p.R = (int)(p.G * a->Sq);
+  n.many = p.R >= kRowsFrom && a->dtype != MLXP_DTYPE_FP32 && a->D >= 64 && a->block_size % kQaTile == 0 &&
+           !a->alibi_slopes;
+  const long long cap = a->max_blocks * a->block_size;
+  if (n.many) {
+    p.rows = std::min(p.R, kQrRows);
+    p.RT = (p.R + kQrRows - 1) / kQrRows;
+    p.HP = 1;
+    p.HG = p.Hk;
+    n.per_sm = 1;
+  } else {
   // 16 rows a warp where there are more than 8 (the codes are then converted once for both
   // halves); the split operands of fp32 leave registers for 8
   n.nt = p.R > 8 && a->dtype != MLXP_DTYPE_FP32 ? 2 : 1;
@@ -82,8 +102,9 @@ QaPlan qa_plan(const mlxp_quant_paged_attn_args* a, int sms, QaParams& p) {
   p.RT = (p.R + 8 * n.nt - 1) / (8 * n.nt);
   p.HP = p.Hk % 4 == 0 ? 4 : p.Hk % 2 == 0 ? 2 : 1;
   p.HG = p.Hk / p.HP;
-  const long long cap = a->max_blocks * a->block_size;
-  const long long chunks = std::max<long long>(1, (cap + kQaChunk - 1) / kQaChunk + 1);
+  }
+  const int chunk = n.many ? kQrKeys : kQaChunk;
+  const long long chunks = std::max<long long>(1, (cap + chunk - 1) / chunk + 1);
   n.grid = std::min<long long>((long long)sms * n.per_sm, (long long)p.B * p.RT * p.HG * chunks);
   const size_t rows = (size_t)n.grid * 2 * p.HP * p.rows;
   n.o_bytes = up256(rows * a->D * 4);
@@ -123,6 +144,22 @@ int qa_maps(const mlxp_quant_paged_attn_args* a, QaMaps& m) {
   return MLXP_OK;
 }
 
+template <typename T, int D>
+int qa_merge(const QaParams& p, long long grid, cudaStream_t s) {
+  if (grid == 1) return MLXP_OK;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(grid - 1), (unsigned)std::min(p.HP * p.rows, 16));
+  cfg.blockDim = dim3(32 * kQaMergeWarps);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, quant_attn_merge_kernel<T, D>, p);
+  return e == cudaSuccess ? MLXP_OK : cuda_fail(e, "quantized paged attention merge launch");
+}
+
 template <typename T, int D, int NT, bool INT8, bool BS16>
 int qa_launch(const QaMaps& maps, const QaParams& p, const QaPlan& n, cudaStream_t s) {
   auto kernel = quant_attn_kernel<T, D, NT, INT8, BS16, qa_min_ctas<D, NT, sizeof(T) == 4>()>;
@@ -139,18 +176,7 @@ int qa_launch(const QaMaps& maps, const QaParams& p, const QaPlan& n, cudaStream
   kernel<<<(unsigned)n.grid, 32 * kQaWarps, smem, s>>>(maps.k, maps.v, p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "quantized paged attention launch");
-  if (n.grid == 1) return MLXP_OK;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(n.grid - 1), (unsigned)std::min(p.HP * p.rows, 16));
-  cfg.blockDim = dim3(32 * kQaMergeWarps);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, quant_attn_merge_kernel<T, D>, p);
-  return e == cudaSuccess ? MLXP_OK : cuda_fail(e, "quantized paged attention merge launch");
+  return qa_merge<T, D>(p, n.grid, s);
 }
 
 template <typename T, int D, int NT>
@@ -161,6 +187,12 @@ int qa_launch_n(const QaMaps& m, const QaParams& p, const QaPlan& n, bool int8, 
 
 template <typename T, int D>
 int qa_launch_d(const QaMaps& m, const QaParams& p, const QaPlan& n, bool int8, cudaStream_t s) {
+  if (n.many) {
+    if (int rc = qa_rows_launch(std::is_same<T, __nv_bfloat16>::value ? MLXP_DTYPE_BF16 : MLXP_DTYPE_FP16, D, int8,
+                                p, (unsigned)n.grid, s))
+      return rc;
+    return qa_merge<T, D>(p, n.grid, s);
+  }
   if constexpr (sizeof(T) == 2)
     if (n.nt == 2) return qa_launch_n<T, D, 2>(m, p, n, int8, s);
   return qa_launch_n<T, D, 1>(m, p, n, int8, s);
@@ -251,6 +283,7 @@ int mlxp_quant_paged_attn(const mlxp_quant_paged_attn_args* a) {
   p.num_blocks = (int)a->num_blocks;
   p.block_size = (int)a->block_size;
   p.max_blocks = (int)a->max_blocks;
+  p.p_scale = n.many ? kQrPScale : kQaPScale;
   p.causal = a->causal ? 1 : 0;
   p.bs_pow2 = (p.block_size & (p.block_size - 1)) == 0;
   p.window = a->window;

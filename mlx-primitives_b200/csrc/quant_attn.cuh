@@ -54,7 +54,7 @@
 namespace mlxp {
 
 constexpr int kQaWarps = 4;
-constexpr int kQaChunk = 64;   // keys a chunk
+constexpr int kQaChunk = 64;   // keys a chunk (quant_attn_rows.cuh: 128)
 constexpr int kQaTile = 16;    // keys a tile
 constexpr float kQaPScale = 32768.f;
 constexpr int kSiteQuantPaged = 12;  // device-status site of this kernel's waits
@@ -88,6 +88,7 @@ struct QaParams {
   int causal, bs_pow2;            // bs_pow2: the block size is a power of two
   long long window;               // -1: none
   float scale_log2;
+  float p_scale;                  // factor of the partials' weights
   int* status;                    // device status word (bounded waits)
   unsigned long long timeout_ns;
 };
@@ -114,7 +115,7 @@ __device__ __forceinline__ void qa_row_range(const QaParams& p, long long ctx, i
   hi = (int)max(h, 0LL);
 }
 
-template <int NT>
+template <int NT, int CHUNK = kQaChunk>
 __device__ __forceinline__ QaRange qa_range(const QaParams& p, int v) {
   QaRange r;
   const int b = v / p.RT, rt = v - b * p.RT;
@@ -134,9 +135,88 @@ __device__ __forceinline__ QaRange qa_range(const QaParams& p, int v) {
       r.fhi = h0;
     }
   }
-  r.c0 = r.klo / kQaChunk;
-  r.n = max(1, (r.khi + kQaChunk - 1) / kQaChunk - r.c0);
+  r.c0 = r.klo / CHUNK;
+  r.n = max(1, (r.khi + CHUNK - 1) / CHUNK - r.c0);
   return r;
+}
+
+// CTA whose range [c * total / grid, (c + 1) * total / grid) holds chunk f.
+__device__ __forceinline__ int qa_cta_of(long long f, long long total, int grid) {
+  return (int)(((f + 1) * grid - 1) / total);
+}
+
+// A CTA's range of chunks: the virtual sequence v and the chunk `rem` of it that chunk f is.
+struct QaWork {
+  long long total, f, f_end, rem;
+  int grid, v;
+  bool any;
+};
+
+// Called by all THREADS of the CTA (at most 1024).
+template <int NT, int CHUNK, int THREADS>
+__device__ __forceinline__ QaWork qa_find_work(const QaParams& p) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ long long s_sum[WARPS], s_rem;
+  __shared__ int s_v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, V = p.B * p.RT;
+  const int per = (V + THREADS - 1) / THREADS;
+  const int va = min(V, (int)threadIdx.x * per), vb = min(V, va + per);
+  long long mine = 0;
+  for (int v = va; v < vb; ++v) mine += (long long)qa_range<NT, CHUNK>(p, v).n * p.HG;
+  long long incl = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += x;
+  }
+  if (lane == 31) s_sum[warp] = incl;
+  __syncthreads();
+  QaWork w;
+  w.total = 0;
+  long long before = incl - mine;
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) {
+    if (i < warp) before += s_sum[i];
+    w.total += s_sum[i];
+  }
+  // no more CTAs than chunks: every working CTA then has some, and a unit's CTAs are consecutive
+  w.grid = (int)min((long long)gridDim.x, w.total);
+  w.f = (long long)blockIdx.x * w.total / w.grid;
+  w.f_end = ((long long)blockIdx.x + 1) * w.total / w.grid;
+  w.any = (int)blockIdx.x < w.grid;
+  if (!w.any) {
+    if (threadIdx.x == 0) p.info[blockIdx.x] = QaPartInfo{-1, 0, 0, 0};
+    return w;
+  }
+  if (w.f >= before && w.f < before + mine) {
+    long long at = before;
+    int v = va;
+    for (; v < vb; ++v) {
+      const long long n = (long long)qa_range<NT, CHUNK>(p, v).n * p.HG;
+      if (w.f < at + n) break;
+      at += n;
+    }
+    s_v = v;
+    s_rem = w.f - at;
+  }
+  __syncthreads();
+  w.v = s_v;
+  w.rem = s_rem;
+  return w;
+}
+
+// What the merge kernel needs of this CTA: the unit of n chunks that its range starts inside of,
+// at chunk ch0 > 0.
+__device__ __forceinline__ void qa_write_info(const QaParams& p, const QaWork& w, int n, int hg, int ch0) {
+  QaPartInfo info{-1, 0, 0, 0};
+  if (ch0 > 0) {
+    const long long u0 = w.f - ch0;  // the unit's first chunk
+    const int first = qa_cta_of(u0, w.total, w.grid);
+    const int last = qa_cta_of(u0 + n - 1, w.total, w.grid);
+    const int slot = (long long)first * w.total / w.grid == u0 ? 0 : 1;
+    info = QaPartInfo{w.v, hg, 2 * first + slot, last - first + 1};
+  }
+  p.info[blockIdx.x] = info;
 }
 
 __device__ __forceinline__ void qa_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -472,11 +552,6 @@ __device__ __forceinline__ void qa_store2(T* p, float a, float b) {
   }
 }
 
-// CTA whose range [c * total / grid, (c + 1) * total / grid) holds chunk f.
-__device__ __forceinline__ int qa_cta_of(long long f, long long total, int grid) {
-  return (int)(((f + 1) * grid - 1) / total);
-}
-
 // Dynamic shared memory of the kernel: the warps' rings, or the warps' merge.
 template <int D, int NT, bool BS16>
 constexpr int qa_smem_bytes() {
@@ -494,10 +569,8 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
   constexpr int RED = D + 4;  // floats a row in the warps' merge: acc, m, l
   __shared__ int s_lo[ROWS], s_hi[ROWS], s_pos[ROWS];
   __shared__ float s_slope[4][ROWS];
-  __shared__ long long s_sum[kQaWarps];
-  __shared__ int s_v, s_abort;
+  __shared__ int s_abort;
   __shared__ __align__(8) uint64_t s_bar[kQaWarps][QaRing<D>::kStages];
-  __shared__ long long s_rem;
   using Q = QaRing<D>;
   extern __shared__ __align__(1024) unsigned char qa_smem[];
   // the warps' rings; between units, the warps' merge ([warp][ROWS][RED] floats)
@@ -524,66 +597,16 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
       tma_prefetch_desc(&tm_v);
     }
   }
-  const int V = p.B * p.RT;
 
-  // this CTA's range: total chunks, then the virtual sequence its first chunk falls in
-  const int per = (V + 32 * kQaWarps - 1) / (32 * kQaWarps);
-  const int va = min(V, (int)threadIdx.x * per), vb = min(V, va + per);
-  long long mine = 0;
-  for (int v = va; v < vb; ++v) mine += (long long)qa_range<NT>(p, v).n * p.HG;
-  long long incl = mine;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, incl, off);
-    if (lane >= off) incl += x;
-  }
-  if (lane == 31) s_sum[warp] = incl;
-  __syncthreads();
-  long long total = 0, before = incl - mine;
-#pragma unroll
-  for (int w = 0; w < kQaWarps; ++w) {
-    if (w < warp) before += s_sum[w];
-    total += s_sum[w];
-  }
-  // no more CTAs than chunks: every working CTA then has some, and a unit's CTAs are consecutive
-  const int grid = (int)min((long long)gridDim.x, total);
-  long long f = (long long)blockIdx.x * total / grid;
-  const long long f_end = ((long long)blockIdx.x + 1) * total / grid;
-  if ((int)blockIdx.x >= grid) {
-    if (threadIdx.x == 0) p.info[blockIdx.x] = QaPartInfo{-1, 0, 0, 0};
-    return;
-  }
-  if (f >= before && f < before + mine) {
-    long long at = before;
-    int v = va;
-    for (; v < vb; ++v) {
-      const long long n = (long long)qa_range<NT>(p, v).n * p.HG;
-      if (f < at + n) break;
-      at += n;
-    }
-    s_v = v;
-    s_rem = f - at;
-  }
-  __syncthreads();
-  int v = s_v;
-  long long rem = s_rem;
-  const long long f_begin = f;
-  while (f < f_end) {
-    const QaRange r = qa_range<NT>(p, v);
-    const int b = v / p.RT, r0 = (v - b * p.RT) * ROWS;
-    const int hg = (int)(rem / r.n), ch0 = (int)(rem - (long long)hg * r.n);
-    const int ch1 = (int)min((long long)r.n, ch0 + (f_end - f));
-    if (f == f_begin && threadIdx.x == 0) {
-      QaPartInfo info{-1, 0, 0, 0};
-      if (ch0 > 0) {
-        const long long u0 = f - ch0;  // the unit's first chunk
-        const int first = qa_cta_of(u0, total, grid);
-        const int last = qa_cta_of(u0 + r.n - 1, total, grid);
-        const int slot = (long long)first * total / grid == u0 ? 0 : 1;
-        info = QaPartInfo{v, hg, 2 * first + slot, last - first + 1};
-      }
-      p.info[blockIdx.x] = info;
-    }
+  QaWork w = qa_find_work<NT, kQaChunk, 32 * kQaWarps>(p);
+  if (!w.any) return;
+  const long long f_begin = w.f;
+  while (w.f < w.f_end) {
+    const QaRange r = qa_range<NT>(p, w.v);
+    const int b = w.v / p.RT, r0 = (w.v - b * p.RT) * ROWS;
+    const int hg = (int)(w.rem / r.n), ch0 = (int)(w.rem - (long long)hg * r.n);
+    const int ch1 = (int)min((long long)r.n, ch0 + (w.f_end - w.f));
+    if (w.f == f_begin && threadIdx.x == 0) qa_write_info(p, w, r.n, hg, ch0);
     __syncthreads();  // the last unit's reads of the row tables and s_red are done
     if (threadIdx.x < ROWS) {
       const int row = r0 + threadIdx.x, i = row / p.G;
@@ -594,9 +617,9 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
       s_pos[threadIdx.x] = (int)(r.ctx - r.qlen + i);
     }
     if (p.alibi && threadIdx.x < HP * ROWS) {
-      const int w = threadIdx.x / ROWS, row = r0 + threadIdx.x % ROWS;
-      s_slope[w][threadIdx.x % ROWS] =
-          row < p.R ? __ldg(p.alibi + (hg * HP + w) * p.G + row % p.G) * 1.4426950408889634f : 0.f;
+      const int hw = threadIdx.x / ROWS, row = r0 + threadIdx.x % ROWS;
+      s_slope[hw][threadIdx.x % ROWS] =
+          row < p.R ? __ldg(p.alibi + (hg * HP + hw) * p.G + row % p.G) * 1.4426950408889634f : 0.f;
     }
     __syncthreads();
     const int hk = hg * HP + hp;
@@ -778,7 +801,7 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
       if (__syncthreads_or(s_abort != 0)) break;  // a wait gave up: nothing more is written
     }
     const bool whole = ch0 == 0 && ch1 == r.n;
-    const long long slot = 2LL * blockIdx.x + (f == f_begin ? 0 : 1);
+    const long long slot = 2LL * blockIdx.x + (w.f == f_begin ? 0 : 1);
     if (KS == 1) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -819,37 +842,37 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
         }
       __syncthreads();
       for (int x = threadIdx.x; x < HP * p.rows * (D / 2); x += blockDim.x) {
-        const int d = 2 * (x % (D / 2)), y = x / (D / 2), tr = y % p.rows, w = y / p.rows;
+        const int d = 2 * (x % (D / 2)), y = x / (D / 2), tr = y % p.rows, hw = y / p.rows;
         const int row = r0 + tr;
         if (row >= p.R) continue;
         float m = -1e30f;
-        for (int k = 0; k < KS; ++k) m = fmaxf(m, s_red[w + k * HP][tr][D]);
+        for (int k = 0; k < KS; ++k) m = fmaxf(m, s_red[hw + k * HP][tr][D]);
         float l = 0.f, a = 0.f, bb = 0.f;
         for (int k = 0; k < KS; ++k) {
-          const float* s = s_red[w + k * HP][tr];
+          const float* s = s_red[hw + k * HP][tr];
           const float wt = ex2_approx(s[D] - m);
           l = fmaf(s[D + 1], wt, l);
           a = fmaf(s[d], wt, a);
           bb = fmaf(s[d + 1], wt, bb);
         }
         if (whole) {
-          const int i = row / p.G, h = (hg * HP + w) * p.G + row - i * p.G;
+          const int i = row / p.G, h = (hg * HP + hw) * p.G + row - i * p.G;
           const bool some = l != 0.f && i < r.qlen;
           const float inv = 1.f / (l * kQaPScale);
           qa_store2<T>(static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh + i * p.o_ss + d,
                        some ? a * inv : 0.f, some ? bb * inv : 0.f);
         } else {
-          const long long pr = (slot * HP + w) * p.rows + tr;
+          const long long pr = (slot * HP + hw) * p.rows + tr;
           *reinterpret_cast<float2*>(p.o_part + pr * D + d) = make_float2(a, bb);
           if (d == 0) *reinterpret_cast<float2*>(p.ml_part + 2 * pr) = make_float2(m, l);
         }
       }
     }
-    f += ch1 - ch0;
-    rem += ch1 - ch0;
-    if (rem >= (long long)r.n * p.HG) {
-      rem = 0;
-      ++v;
+    w.f += ch1 - ch0;
+    w.rem += ch1 - ch0;
+    if (w.rem >= (long long)r.n * p.HG) {
+      w.rem = 0;
+      ++w.v;
     }
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -922,7 +945,7 @@ __global__ void __launch_bounds__(32 * kQaMergeWarps) quant_attn_merge_kernel(co
       }
       const int i = row / p.G, h = (info.hg * p.HP + w) * p.G + row - i * p.G;
       const bool some = lt != 0.f && i < qlen;
-      const float inv = 1.f / (lt * kQaPScale);
+      const float inv = 1.f / (lt * p.p_scale);
       qa_store2<T>(static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh + i * p.o_ss + 2 * threadIdx.x,
                    some ? x * inv : 0.f, some ? z * inv : 0.f);
     }
