@@ -879,7 +879,9 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
 }
 
 // Merges the partials of the units that more than one CTA worked on.  Block x looks at main CTA
-// x + 1: where that is the second CTA of a unit, it merges the unit's rows blockIdx.y, +gridDim.y...
+// x + 1: where that is the second CTA of a unit, it merges the unit's rows.  Up to 32 partials a
+// warp takes a row to itself; the rows of a unit split further (few units, long contexts) are
+// taken by all the block's warps together.
 constexpr int kQaMergeWarps = 8;
 
 template <typename T, int D>
@@ -895,7 +897,10 @@ __global__ void __launch_bounds__(32 * kQaMergeWarps) quant_attn_merge_kernel(co
   const int sub = lane / LPR, d = (lane % LPR) * 4;
   const int b = info.v / p.RT, r0 = (info.v - b * p.RT) * p.rows;
   const int qlen = p.query_lens ? p.query_lens[b] : p.Sq;
-  for (int y = blockIdx.y; y < p.HP * p.rows; y += gridDim.y) {
+  const bool together = info.parts > 32;
+  const int team = together ? kQaMergeWarps : 1, me = together ? warp : 0;  // warps a row, this one's place
+  const int stride = together ? gridDim.y : gridDim.y * kQaMergeWarps;
+  for (int y = together ? blockIdx.y : blockIdx.y * kQaMergeWarps + warp; y < p.HP * p.rows; y += stride) {
     const int tr = y % p.rows, w = y / p.rows, row = r0 + tr;
     if (row >= p.R) continue;
     auto at = [&](int j) {  // partial row of the unit's j-th CTA
@@ -903,17 +908,19 @@ __global__ void __launch_bounds__(32 * kQaMergeWarps) quant_attn_merge_kernel(co
       return (slot * p.HP + w) * p.rows + tr;
     };
     float m = -1e30f;
-    for (int j = threadIdx.x; j < info.parts; j += 32 * kQaMergeWarps) m = fmaxf(m, p.ml_part[2 * at(j)]);
+    for (int j = me * 32 + lane; j < info.parts; j += 32 * team) m = fmaxf(m, p.ml_part[2 * at(j)]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-    if (lane == 0) s_m[warp] = m;
-    __syncthreads();
+    if (together) {
+      if (lane == 0) s_m[warp] = m;
+      __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kQaMergeWarps; ++k) m = fmaxf(m, s_m[k]);
+      for (int k = 0; k < kQaMergeWarps; ++k) m = fmaxf(m, s_m[k]);
+    }
     float l = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int j = warp * PPW + sub; j < info.parts; j += kQaMergeWarps * PPW) {
+    for (int j = me * PPW + sub; j < info.parts; j += team * PPW) {
       const long long pr = at(j);
       const float2 ml = *reinterpret_cast<const float2*>(p.ml_part + 2 * pr);
       const float4 o = *reinterpret_cast<const float4*>(p.o_part + pr * D + d);
@@ -932,24 +939,31 @@ __global__ void __launch_bounds__(32 * kQaMergeWarps) quant_attn_merge_kernel(co
       a.z += __shfl_xor_sync(0xffffffffu, a.z, off);
       a.w += __shfl_xor_sync(0xffffffffu, a.w, off);
     }
-    if (sub == 0) *reinterpret_cast<float4*>(&s_o[warp][d]) = a;
-    if (lane == 0) s_l[warp] = l;
-    __syncthreads();
-    if (threadIdx.x < D / 2) {
-      float x = 0.f, z = 0.f, lt = 0.f;
+    if (together) {
+      if (sub == 0) *reinterpret_cast<float4*>(&s_o[warp][d]) = a;
+      if (lane == 0) s_l[warp] = l;
+      __syncthreads();
+      a = make_float4(0.f, 0.f, 0.f, 0.f);
+      l = 0.f;
 #pragma unroll
       for (int k = 0; k < kQaMergeWarps; ++k) {
-        x += s_o[k][2 * threadIdx.x];
-        z += s_o[k][2 * threadIdx.x + 1];
-        lt += s_l[k];
+        const float4 x = *reinterpret_cast<const float4*>(&s_o[k][d]);
+        a.x += x.x;
+        a.y += x.y;
+        a.z += x.z;
+        a.w += x.w;
+        l += s_l[k];
       }
-      const int i = row / p.G, h = (info.hg * p.HP + w) * p.G + row - i * p.G;
-      const bool some = lt != 0.f && i < qlen;
-      const float inv = 1.f / (lt * p.p_scale);
-      qa_store2<T>(static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh + i * p.o_ss + 2 * threadIdx.x,
-                   some ? x * inv : 0.f, some ? z * inv : 0.f);
     }
-    __syncthreads();
+    if (sub == 0 && me == 0) {
+      const int i = row / p.G, h = (info.hg * p.HP + w) * p.G + row - i * p.G;
+      const bool some = l != 0.f && i < qlen;
+      const float inv = 1.f / (l * p.p_scale);
+      T* o = static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh + i * p.o_ss + d;
+      qa_store2<T>(o, some ? a.x * inv : 0.f, some ? a.y * inv : 0.f);
+      qa_store2<T>(o + 2, some ? a.z * inv : 0.f, some ? a.w * inv : 0.f);
+    }
+    if (together) __syncthreads();
   }
 }
 

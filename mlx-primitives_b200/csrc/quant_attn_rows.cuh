@@ -35,6 +35,11 @@ constexpr int kQrThreads = 512;
 constexpr int kQrRows = 256, kQrKeys = 128;
 constexpr float kQrPScale = 4096.f;
 constexpr float kQrHeadroom = 3.f;
+#ifndef QR_POLY
+#define QR_POLY 2
+#endif
+// of every 8 pairs of weights, exponentiated on the FMA pipe (exp2_poly2, 7.2e-5 off at most)
+constexpr int kQrPolyPerOct = QR_POLY;
 constexpr int kSiteQuantRows = 13;
 // registers a thread of the softmax, converting and issuing warpgroups: 128 * (2 * 184 + 104 + 40)
 // = 65536 = what 512 threads of 128 are launched with
@@ -270,8 +275,12 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
               const float f = fmaxf(sc[g].x * qs, 1.2e-38f), vs = sc[g].z;  // > 0: -inf stays -inf
               const float2 x = fma2(make_float2(s[64 * hf + 2 * e], s[64 * hf + 2 * e + 1]), make_float2(f, f), negm);
               float2 y;
-              y.x = ex2_approx(x.x);
-              y.y = ex2_approx(x.y);
+              if ((e & 7) < kQrPolyPerOct) {
+                y = exp2_poly2(x);
+              } else {
+                y.x = ex2_approx(x.x);
+                y.y = ex2_approx(x.y);
+              }
               acc = add2(acc, y);
               y = mul2(y, make_float2(vs, vs));
               pk[e] = qa_pack(y.x, y.y);
@@ -343,42 +352,56 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
       const Unit u = next_unit();
       __syncthreads();
       const int* bt = p.block_tables + (long long)u.b * p.bt_stride;
-      const long long head = (long long)u.hk * p.p_sh + 16 * l;
-      // the block of 16-key group g of this warp's two in tile j, -1 without keys
-      auto block_of = [&](int j, int g) {
-        const int key = (u.r.c0 + j) * kQrKeys + 32 * cw + 16 * g;
-        if (j >= u.ch1 || key >= u.r.khi) return -1;
-        const int id = __ldg(bt + (unsigned)key / (unsigned)p.block_size);
-        return id < p.num_blocks ? id : -1;
+      const long long mine = (long long)u.hk * p.p_sh + rr * p.p_st + 16 * l;  // this lane's piece of row 0
+      // A 16-key group of this warp's two in a tile: its pool block and first row's offset, and
+      // how many of its rows are keys.
+      struct Group {
+        int id, rows;
+        long long off;
       };
-      auto load = [&](const unsigned char* pool, int j, int id0, int id1, uint4 (&x)[IT]) {
-        const int key0 = (u.r.c0 + j) * kQrKeys + 32 * cw;
+      auto group = [&](int j, int g) {
+        Group x{-1, 0, 0};
+        const int key = (u.r.c0 + j) * kQrKeys + 32 * cw + 16 * g;
+        if (j >= u.ch1 || key >= u.r.khi) return x;
+        const unsigned slot = (unsigned)key / (unsigned)p.block_size;
+        const int id = __ldg(bt + slot);
+        if (id < 0 || id >= p.num_blocks) return x;
+        x.id = id;
+        x.rows = min(16, u.r.khi - key);
+        x.off = (long long)id * p.p_sb + (long long)(key - (int)slot * p.block_size) * p.p_st + mine;
+        return x;
+      };
+      auto load = [&](const unsigned char* pool, const Group& g0, const Group& g1, uint4 (&x)[IT]) {
+        const unsigned char* q0 = pool + g0.off;
+        const unsigned char* q1 = pool + g1.off;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-          const int k = i * RPI + rr, id = k < 16 ? id0 : id1;
+          const int k = (i % (IT / 2)) * RPI;  // the piece's row in its group, less rr
           x[i] = make_uint4(0, 0, 0, 0);
-          if (id >= 0 && key0 + k < u.r.khi) {
-            const unsigned in = (unsigned)(key0 + (k & ~15)) % (unsigned)p.block_size + (k & 15);
-            x[i] = __ldg(reinterpret_cast<const uint4*>(pool + (long long)id * p.p_sb + in * p.p_st + head));
-          }
+          if (k + rr < (i < IT / 2 ? g0.rows : g1.rows))
+            x[i] = __ldg(reinterpret_cast<const uint4*>((i < IT / 2 ? q0 : q1) + k * p.p_st));
         }
       };
-      int a0 = block_of(u.ch0, 0), a1 = block_of(u.ch0, 1);
-      int b0 = block_of(u.ch0 + 1, 0), b1 = block_of(u.ch0 + 1, 1);
+      // lanes 0 and 1 hold the scales of the two groups
+      auto scales = [&](const Group& g0, const Group& g1, float& ks, float& vs) {
+        const int id = lane == 0 ? g0.id : lane == 1 ? g1.id : -1;
+        ks = vs = 0.f;
+        if (id < 0) return;
+        const long long at = (long long)id * p.sc_sb + (long long)u.hk * p.sc_sh;
+        ks = __ldg(p.k_scales + at);
+        vs = __ldg(p.v_scales + at);
+      };
+      Group a0 = group(u.ch0, 0), a1 = group(u.ch0, 1);  // of tile j, and of j + 1
+      Group b0 = group(u.ch0 + 1, 0), b1 = group(u.ch0 + 1, 1);
       uint4 kx[IT], vx[IT];
-      load(p.k_pool, u.ch0, a0, a1, kx);
-      load(p.v_pool, u.ch0, a0, a1, vx);
+      float ks, vs, ks_next, vs_next;
+      load(p.k_pool, a0, a1, kx);
+      load(p.v_pool, a0, a1, vx);
+      scales(a0, a1, ks, vs);
       bool ok = true;
       for (int j = u.ch0; j < u.ch1; ++j) {
         const int c = cnt + j - u.ch0, st = c & 1;
-        // this warp's groups' scales (lanes 0, 1), and whether they have blocks
-        float ks = 0.f, vs = 0.f;
-        const int mine = lane == 0 ? a0 : lane == 1 ? a1 : -1;
-        if (mine >= 0) {
-          const long long at = (long long)mine * p.sc_sb + (long long)u.hk * p.sc_sh;
-          ks = __ldg(p.k_scales + at);
-          vs = __ldg(p.v_scales + at);
-        }
+        scales(b0, b1, ks_next, vs_next);
         const uint32_t neg = __ballot_sync(0xffffffffu, ks < 0.f);
         if (c >= 2) {
           ok = __all_sync(0xffffffffu, mbar_wait(BAR(C::B_KE + st), (c / 2 - 1) & 1, wctx, kSiteQuantRows));
@@ -389,7 +412,7 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
               make_float4(fmaxf(fabsf(ks), 7.5e-37f), qa_log_scale(vs), vs * kQrPScale, 0.f);
         }
         if (lane == 2)
-          (smem + C::OFF_MASK)[(c & 3) * 4 + cw] = (unsigned char)((a0 >= 0) | (a1 >= 0) << 1);
+          (smem + C::OFF_MASK)[(c & 3) * 4 + cw] = (unsigned char)((a0.id >= 0) | (a1.id >= 0) << 1);
         const uint32_t kt = sbase + C::OFF_K + st * C::TILE;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
@@ -399,7 +422,7 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(BAR(C::B_KF + st));
-        if (j + 1 < u.ch1) load(p.k_pool, j + 1, b0, b1, kx);
+        load(p.k_pool, b0, b1, kx);
         if (c >= 2) {
           ok = __all_sync(0xffffffffu, mbar_wait(BAR(C::B_VE + st), (c / 2 - 1) & 1, wctx, kSiteQuantRows));
           if (!ok) break;
@@ -410,11 +433,13 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(BAR(C::B_VF + st));
-        if (j + 1 < u.ch1) load(p.v_pool, j + 1, b0, b1, vx);
+        load(p.v_pool, b0, b1, vx);
         a0 = b0;
         a1 = b1;
-        b0 = block_of(j + 2, 0);
-        b1 = block_of(j + 2, 1);
+        b0 = group(j + 2, 0);
+        b1 = group(j + 2, 1);
+        ks = ks_next;
+        vs = vs_next;
       }
       cnt += u.ch1 - u.ch0;
       if (__syncthreads_or(s_abort != 0)) break;
