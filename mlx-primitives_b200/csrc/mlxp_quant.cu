@@ -283,7 +283,7 @@ int mlxp_quant_paged_attn(const mlxp_quant_paged_attn_args* a) {
   p.num_blocks = (int)a->num_blocks;
   p.block_size = (int)a->block_size;
   p.max_blocks = (int)a->max_blocks;
-  p.p_scale = n.many ? kQrPScale : kQaPScale;
+  p.p_scale = n.many ? 1.f : kQaPScale;
   p.causal = a->causal ? 1 : 0;
   p.bs_pow2 = (p.block_size & (p.block_size - 1)) == 0;
   p.window = a->window;
