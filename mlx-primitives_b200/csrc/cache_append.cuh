@@ -20,9 +20,10 @@
 // in int8.
 //
 // One unit is (sequence, touched block, head, K or V), taken by WPU warps: they read the block's
-// new rows once, keep the rotated values in registers (32 a lane: 8 rows of 128 a warp), agree
-// on amax through shared memory and write the codes.  A block of more rows than the warps hold is
-// read a second time (from L2) instead.  Bound by HBM for prompts, by latency for single tokens.
+// new rows once and keep them in registers (16 bf16 rows of 128 a warp: blocks of 16 need no other
+// warp), compute their values twice, for amax and for the codes, and agree on amax through shared
+// memory where they are several.  A block of more rows than eight warps hold is read a second time
+// (from L2).  Bound by HBM for prompts, by latency for single tokens.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -109,6 +110,14 @@ __device__ __forceinline__ void append_q_unit(const AppendParams& p, unsigned u,
     if (h0 >= last) return;
     load(h0);
   }
+}
+
+// Query units alone (many of them, beside an 8-bit pool's block units in another launch).
+template <typename R, int U>
+__global__ void __launch_bounds__(256, 3) append_q_kernel(const AppendParams p) {
+  const int lane = threadIdx.x & 31, j = lane % R::LPR, g = lane / R::LPR;
+  for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < p.q_units; u += 8LL * gridDim.x)
+    append_q_unit<R, U>(p, (unsigned)u, j, g);
 }
 
 // Pools of the inputs' type: units [0, q_units) are queries, then keys, then values.
@@ -212,14 +221,12 @@ __device__ __forceinline__ void store_codes(unsigned char* y, const float* x) {
   }
 }
 
-template <typename R>
-__host__ __device__ constexpr int append_steps() { return 32 / (2 * R::NE); }  // row steps a warp keeps
+constexpr int kAppendSteps = 4;           // row steps of a block that a warp keeps
 
 template <typename R, int U, bool INT8>
 __global__ void __launch_bounds__(256, 2) append_quant_kernel(const AppendParams p) {
   using T = typename R::T;
-  constexpr int STEPS = append_steps<R>();
-  constexpr int ROWS = STEPS * R::RPW;    // rows a warp keeps
+  constexpr int ROWS = kAppendSteps * R::RPW;  // rows a warp keeps
   __shared__ float s_amax[8];
   const int lane = threadIdx.x & 31, j = lane % R::LPR, g = lane / R::LPR;
   const int warp = threadIdx.x >> 5;
@@ -234,8 +241,8 @@ __global__ void __launch_bounds__(256, 2) append_quant_kernel(const AppendParams
   for (long long u0 = (long long)(blockIdx.x - p.q_ctas) * upc; u0 < p.block_units; u0 += ctas * upc) {
     const long long u = u0 + warp / p.wpu;
     // unit = ((sequence * touch + slot) * 2 + is_v) * Hk + head
-    bool on = u < p.block_units;
-    const unsigned uu = (unsigned)(on ? u : 0);
+    const bool there = u < p.block_units;
+    const unsigned uu = (unsigned)(there ? u : 0);
     const int h = (int)(uu % (unsigned)p.Hk);
     const unsigned rest = uu / (unsigned)p.Hk;
     const bool is_v = rest & 1;
@@ -246,22 +253,36 @@ __global__ void __launch_bounds__(256, 2) append_quant_kernel(const AppendParams
     const long long lo = ctx < 0 ? 0 : ctx, hi = ctx + append_count(p, b);  // new positions
     const long long slot = lo / p.block_size + slot_i, base = slot * p.block_size;
     const int r0 = (int)max(lo - base, 0LL);                        // new rows of the block
-    const int r1 = (int)min(hi - base, (long long)p.block_size);
-    int id = -1;
-    if (on && hi > lo && r0 < r1) id = pool_block(p, b, slot);
-    on = id >= 0;
+    // none where the block is past the table: so are its positions, which the cos/sin tables need
+    // not cover
+    const int r1 = there && hi > lo && slot < p.max_blocks
+                       ? (int)max(min(hi - base, (long long)p.block_size), (long long)r0)
+                       : r0;
+    const int stride = ROWS * p.wpu;      // rows the unit's warps hold at a time
+    // slabs of `stride` rows that hold new ones: [first, first + n) of the block's
+    const int first = r0 / stride, n = r1 > r0 ? (r1 - 1) / stride - first + 1 : 0;
+    if (p.wpu == 1 && n == 0) continue;   // the same for the whole warp, which syncs with none
     const long long* st = is_v ? p.v_s : p.k_s;
     const T* x = static_cast<const T*>(is_v ? p.v : p.k) + b * st[0] + h * st[1];
+    // The rows are on their way before the block is known.
+    RowData<R> d[kAppendSteps];
+    auto load = [&](int sl) {
+      const int row0 = (first + sl) * stride + part * ROWS + g;
+#pragma unroll
+      for (int i = 0; i < kAppendSteps; ++i) {
+        const int r = row0 + i * R::RPW;
+        row_load<R>(x + (base + r - ctx) * st[2], p.half, j, r >= r0 && r < r1, d[i]);
+      }
+    };
+    if (n > 0) load(0);
+    const int id = n > 0 ? pool_block(p, b, slot) : -1;
+    const bool on = id >= 0;
     unsigned char* pool = static_cast<unsigned char*>(is_v ? p.v_pool : p.k_pool) +
                           (on ? id : 0) * p.p_sb + h * p.p_sh;
     float* scale = (is_v ? p.v_scales : p.k_scales) + (on ? id : 0) * p.sc_sb + h * p.sc_sh;
-    const float s_old = on ? *scale : 1.f;
-    const int stride = ROWS * p.wpu;      // rows the unit's warps hold at a time
-    // slabs of `stride` rows that hold new ones: [first, first + n) of the block's
-    const int first = r0 / stride, n = on ? (r1 - 1) / stride - first + 1 : 0;
+    const float s_old = on && r0 > 0 ? *scale : 0.f;
     RowCoef<R> kw;
-    if (on && !is_v) coef_weights<R>(p.k_norm, p.half, j, kw);
-    float2 y1[STEPS][R::NP], y2[STEPS][R::NP];
+    if (!is_v) coef_weights<R>(p.k_norm, p.half, j, kw);
     float s_new = 1.f;
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
@@ -270,50 +291,40 @@ __global__ void __launch_bounds__(256, 2) append_quant_kernel(const AppendParams
       const float inv = pass == 1 && !divide ? __fdiv_rn(1.f, s_new) : 1.f;
 #pragma unroll 1
       for (int sl = 0; sl < n; ++sl) {
+        if (n > 1 && (pass == 1 || sl > 0)) load(sl);
         const int row0 = (first + sl) * stride + part * ROWS + g;
-        if (pass == 0 || n > 1) {
-          RowData<R> d[STEPS];
 #pragma unroll
-          for (int i = 0; i < STEPS; ++i) {
-            const int r = row0 + i * R::RPW;
-            row_load<R>(x + (base + r - ctx) * st[2], p.half, j, r >= r0 && r < r1, d[i]);
-          }
-#pragma unroll
-          for (int i = 0; i < STEPS; ++i) {
-            const int r = row0 + i * R::RPW;
-            const bool live = r >= r0 && r < r1;
-            if (is_v) {
-              row_to_f<R>(d[i].x1, y1[i]);
-              row_to_f<R>(d[i].x2, y2[i]);
-            } else if (__any_sync(0xffffffffu, live)) {
-              coef_tables<R>(p.cosc, p.sinc, live ? base + r : 0, p.half, j, kw);
-              row_norm_rope<R>(d[i], p.k_norm, p.cosc != nullptr, kw, y1[i], y2[i]);
-            } else {
-              fill2<R::NP>(0.f, y1[i], y2[i]);
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
+        for (int i = 0; i < kAppendSteps; ++i) {
           const int r = row0 + i * R::RPW;
           const bool live = r >= r0 && r < r1;
+          if (!__any_sync(0xffffffffu, live)) continue;
+          // the rows' values, computed again in the second pass: kept, they would be twice the
+          // registers of the rows themselves
+          float2 y1[R::NP], y2[R::NP];
+          if (is_v) {
+            row_to_f<R>(d[i].x1, y1);
+            row_to_f<R>(d[i].x2, y2);
+          } else {
+            coef_tables<R>(p.cosc, p.sinc, live ? base + r : 0, p.half, j, kw);
+            row_norm_rope<R>(d[i], p.k_norm, p.cosc != nullptr, kw, y1, y2);
+          }
           if (pass == 0) {
             // the largest first; where it is not finite, the finite ones one by one (the maximum
             // passes NaN over, which the clamp's code keeps)
             float big = 0.f;
 #pragma unroll
             for (int e = 0; e < R::NP; ++e)
-              big = fmaxf(fmaxf(big, fmaxf(fabsf(y1[i][e].x), fabsf(y1[i][e].y))),
-                          fmaxf(fabsf(y2[i][e].x), fabsf(y2[i][e].y)));
+              big = fmaxf(fmaxf(big, fmaxf(fabsf(y1[e].x), fabsf(y1[e].y))),
+                          fmaxf(fabsf(y2[e].x), fabsf(y2[e].y)));
             if (big > 3.402823466e38f) {
               big = 0.f;
 #pragma unroll
               for (int e = 0; e < R::NP; ++e)
-                for (const float a : {y1[i][e].x, y1[i][e].y, y2[i][e].x, y2[i][e].y})
+                for (const float a : {y1[e].x, y1[e].y, y2[e].x, y2[e].y})
                   if (fabsf(a) <= 3.402823466e38f) big = fmaxf(big, fabsf(a));
             }
             if (live) amax = fmaxf(amax, big);
-          } else if (live) {
+          } else if (live && on) {
 #pragma unroll
             for (int c = 0; c < R::NC; ++c) {
               const int at = piece_at<R>(c, j);
@@ -321,9 +332,9 @@ __global__ void __launch_bounds__(256, 2) append_quant_kernel(const AppendParams
               float a[R::VEC], e2[R::VEC];
 #pragma unroll
               for (int e = 0; e < R::VEC; ++e) {
-                const int x = c * R::VEC + e;
-                const float f1 = x & 1 ? y1[i][x / 2].y : y1[i][x / 2].x;
-                const float f2 = x & 1 ? y2[i][x / 2].y : y2[i][x / 2].x;
+                const int z = c * R::VEC + e;
+                const float f1 = z & 1 ? y1[z / 2].y : y1[z / 2].x;
+                const float f2 = z & 1 ? y2[z / 2].y : y2[z / 2].x;
                 a[e] = divide ? __fdiv_rn(f1, s_new) : f1 * inv;
                 e2[e] = divide ? __fdiv_rn(f2, s_new) : f2 * inv;
               }

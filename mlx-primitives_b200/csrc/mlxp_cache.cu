@@ -74,6 +74,11 @@ constexpr int fwd_steps() { return 2; }
 template <typename R>
 constexpr int bwd_steps() { return R::kWide ? 2 : 1; }
 
+// From this many query units an SM, appends to 8-bit pools take two launches: the query rows run
+// at three CTAs an SM in a kernel of their own, at two beside the block units, whose registers
+// they share (8 ragged prompts, 17.6 K tokens of 32 + 2 x 8 heads of 128: 173 us in one launch).
+constexpr long long kSplitUnits = 64;
+
 int launched(const char* what) {
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MLXP_OK : cuda_fail(e, what);
@@ -350,7 +355,7 @@ int mlxp_paged_append(const mlxp_paged_append_args* a) {
       return launched("paged_append launch");
     }
     // warps a unit: as many as hold the rows it can have, at most all eight
-    constexpr int ROWS = append_steps<R>() * R::RPW;
+    constexpr int ROWS = kAppendSteps * R::RPW;
     const long long rows = std::min<long long>(a->block_size, a->S);
     p.wpu = 1;
     while (p.wpu < 8 && p.wpu * ROWS < rows) p.wpu *= 2;
@@ -358,6 +363,11 @@ int mlxp_paged_append(const mlxp_paged_append_args* a) {
     p.block_units = a->B * p.touch * 2 * a->Hk;
     if (p.block_units > INT32_MAX) return fail(MLXP_ERR_INVALID, "paged shape too large");
     const int upc = 8 / p.wpu;
+    if (p.q_units >= kSplitUnits * sms) {  // many query rows: a launch of their own, see there
+      append_q_kernel<R, U><<<(unsigned)std::min<long long>((p.q_units + 7) / 8, 64LL * sms), 256, 0, s>>>(p);
+      if (int rc = launched("paged_append launch (queries)")) return rc;
+      p.q_units = 0;
+    }
     p.q_ctas = (int)std::min<long long>((p.q_units + 7) / 8, 16LL * sms);
     const long long ctas = std::min<long long>((p.block_units + upc - 1) / upc, 64LL * sms);
     const unsigned grid = (unsigned)(p.q_ctas + ctas);
