@@ -20,9 +20,9 @@
 // in int8.
 //
 // One unit is (sequence, touched block, head, K or V), taken by WPU warps: they read the block's
-// new rows once and keep them in registers (16 bf16 rows of 128 a warp: blocks of 16 need no other
-// warp), compute their values twice, for amax and for the codes, and agree on amax through shared
-// memory where they are several.  A block of more rows than eight warps hold is read a second time
+// new rows once and keep them (16 bf16 rows of 128 a warp: blocks of 16 need no other warp), in
+// registers, the keys' computed values in shared memory, until amax is known, on which they agree
+// through shared memory where they are several.  A block of more rows than eight warps hold is read a second time
 // (from L2).  Bound by HBM for prompts, by latency for single tokens.
 #pragma once
 
@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(256, 2) append_quant_kernel(const AppendParams
   using T = typename R::T;
   constexpr int ROWS = kAppendSteps * R::RPW;  // rows a warp keeps
   __shared__ float s_amax[8];
+  extern __shared__ float4 s_keep[];      // [8 warps][kAppendSteps][NP][32 lanes]
   const int lane = threadIdx.x & 31, j = lane % R::LPR, g = lane / R::LPR;
   const int warp = threadIdx.x >> 5;
   if ((int)blockIdx.x < p.q_ctas) {
@@ -298,15 +299,27 @@ __global__ void __launch_bounds__(256, 2) append_quant_kernel(const AppendParams
           const int r = row0 + i * R::RPW;
           const bool live = r >= r0 && r < r1;
           if (!__any_sync(0xffffffffu, live)) continue;
-          // the rows' values, computed again in the second pass: kept, they would be twice the
-          // registers of the rows themselves
+          // A key's values wait in shared memory for the second pass (every lane's own, so without
+          // a barrier): in registers they would take twice the rows' room.
           float2 y1[R::NP], y2[R::NP];
+          float4* keep = s_keep + (warp * kAppendSteps + i) * R::NP * 32 + lane;
           if (is_v) {
             row_to_f<R>(d[i].x1, y1);
             row_to_f<R>(d[i].x2, y2);
-          } else {
+          } else if (pass == 0 || n > 1) {
             coef_tables<R>(p.cosc, p.sinc, live ? base + r : 0, p.half, j, kw);
             row_norm_rope<R>(d[i], p.k_norm, p.cosc != nullptr, kw, y1, y2);
+            if (pass == 0) {
+#pragma unroll
+              for (int e = 0; e < R::NP; ++e) keep[32 * e] = make_float4(y1[e].x, y1[e].y, y2[e].x, y2[e].y);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < R::NP; ++e) {
+              const float4 z = keep[32 * e];
+              y1[e] = make_float2(z.x, z.y);
+              y2[e] = make_float2(z.z, z.w);
+            }
           }
           if (pass == 0) {
             // the largest first; where it is not finite, the finite ones one by one (the maximum

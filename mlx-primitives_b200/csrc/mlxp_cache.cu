@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "../../include/mlxp_attn.h"
@@ -82,6 +83,22 @@ constexpr long long kSplitUnits = 64;
 int launched(const char* what) {
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MLXP_OK : cuda_fail(e, what);
+}
+
+template <typename R, int U, bool INT8>
+int append_quant_launch(const AppendParams& p, unsigned grid, cudaStream_t s) {
+  constexpr int smem = 8 * kAppendSteps * R::NP * 32 * (int)sizeof(float4);
+  static std::atomic<unsigned long long> attr_done{0};  // one bit per device
+  int dev;
+  if (int rc = current_device(dev)) return rc;
+  if (!(attr_done.load() >> dev & 1ull)) {
+    const cudaError_t e = cudaFuncSetAttribute(append_quant_kernel<R, U, INT8>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_append)");
+    attr_done.fetch_or(1ull << dev);
+  }
+  append_quant_kernel<R, U, INT8><<<grid, 256, smem, s>>>(p);
+  return launched("paged_append launch");
 }
 
 int norm_rope_check(const mlxp_qk_norm_rope_args* a, bool bwd) {
@@ -371,9 +388,8 @@ int mlxp_paged_append(const mlxp_paged_append_args* a) {
     p.q_ctas = (int)std::min<long long>((p.q_units + 7) / 8, 16LL * sms);
     const long long ctas = std::min<long long>((p.block_units + upc - 1) / upc, 64LL * sms);
     const unsigned grid = (unsigned)(p.q_ctas + ctas);
-    if (a->cache_dtype == MLXP_DTYPE_INT8) append_quant_kernel<R, U, true><<<grid, 256, 0, s>>>(p);
-    else append_quant_kernel<R, U, false><<<grid, 256, 0, s>>>(p);
-    return launched("paged_append launch");
+    return a->cache_dtype == MLXP_DTYPE_INT8 ? append_quant_launch<R, U, true>(p, grid, s)
+                                             : append_quant_launch<R, U, false>(p, grid, s);
   });
 }
 
