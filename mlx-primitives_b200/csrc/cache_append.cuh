@@ -21,7 +21,7 @@
 //
 // One unit is (sequence, touched block, head, K or V), taken by WPU warps: they read the block's
 // new rows once and keep them (16 bf16 rows of 128 a warp: blocks of 16 need no other warp), in
-// registers, the keys' computed values in shared memory, until amax is known, on which they agree
+// registers as loaded and in shared memory as computed, until amax is known, on which they agree
 // through shared memory where they are several.  A block of more rows than eight warps hold is read a second time
 // (from L2).  Bound by HBM for prompts, by latency for single tokens.
 #pragma once
@@ -285,6 +285,9 @@ __global__ void __launch_bounds__(256, 2) append_quant_kernel(const AppendParams
     RowCoef<R> kw;
     if (!is_v) coef_weights<R>(p.k_norm, p.half, j, kw);
     float s_new = 1.f;
+    // The rows' values wait in shared memory for the block's scale, every lane's own, so without a
+    // barrier: in registers they would take twice the rows' room.
+    float4* mine = s_keep + warp * kAppendSteps * R::NP * 32 + lane;
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
       float amax = 0.f;
@@ -294,67 +297,83 @@ __global__ void __launch_bounds__(256, 2) append_quant_kernel(const AppendParams
       for (int sl = 0; sl < n; ++sl) {
         if (n > 1 && (pass == 1 || sl > 0)) load(sl);
         const int row0 = (first + sl) * stride + part * ROWS + g;
+        if (pass == 0 || n > 1) {
 #pragma unroll
+          for (int i = 0; i < kAppendSteps; ++i) {
+            const int r = row0 + i * R::RPW;
+            const bool live = r >= r0 && r < r1;
+            if (!__any_sync(0xffffffffu, live)) continue;
+            float2 y1[R::NP], y2[R::NP];
+            if (is_v) {
+              row_to_f<R>(d[i].x1, y1);
+              row_to_f<R>(d[i].x2, y2);
+            } else {
+              coef_tables<R>(p.cosc, p.sinc, live ? base + r : 0, p.half, j, kw);
+              row_norm_rope<R>(d[i], p.k_norm, p.cosc != nullptr, kw, y1, y2);
+            }
+            float4* keep = mine + i * R::NP * 32;
+            float big = 0.f;
+#pragma unroll
+            for (int e = 0; e < R::NP; ++e) {
+              keep[32 * e] = make_float4(y1[e].x, y1[e].y, y2[e].x, y2[e].y);
+              big = fmaxf(fmaxf(big, fmaxf(fabsf(y1[e].x), fabsf(y1[e].y))),
+                          fmaxf(fabsf(y2[e].x), fabsf(y2[e].y)));
+            }
+            if (big > 3.402823466e38f) {  // infinities: the finite ones one by one
+              big = 0.f;
+#pragma unroll 1
+              for (int e = 0; e < R::NP; ++e) {
+                const float4 z = keep[32 * e];
+                for (const float v : {z.x, z.y, z.z, z.w})
+                  if (fabsf(v) <= 3.402823466e38f) big = fmaxf(big, fabsf(v));
+              }
+            }
+            if (live) amax = fmaxf(amax, big);  // fmaxf passes NaN over
+          }
+        }
+        if (pass == 0 || !on) continue;
+#pragma unroll 1
         for (int i = 0; i < kAppendSteps; ++i) {
           const int r = row0 + i * R::RPW;
-          const bool live = r >= r0 && r < r1;
-          if (!__any_sync(0xffffffffu, live)) continue;
-          // A key's values wait in shared memory for the second pass (every lane's own, so without
-          // a barrier): in registers they would take twice the rows' room.
-          float2 y1[R::NP], y2[R::NP];
-          float4* keep = s_keep + (warp * kAppendSteps + i) * R::NP * 32 + lane;
-          if (is_v) {
-            row_to_f<R>(d[i].x1, y1);
-            row_to_f<R>(d[i].x2, y2);
-          } else if (pass == 0 || n > 1) {
-            coef_tables<R>(p.cosc, p.sinc, live ? base + r : 0, p.half, j, kw);
-            row_norm_rope<R>(d[i], p.k_norm, p.cosc != nullptr, kw, y1, y2);
-            if (pass == 0) {
+          if (r < r0 || r >= r1) continue;
+          const float4* keep = mine + i * R::NP * 32;
+          float v1[R::NE], v2[R::NE];
 #pragma unroll
-              for (int e = 0; e < R::NP; ++e) keep[32 * e] = make_float4(y1[e].x, y1[e].y, y2[e].x, y2[e].y);
+          for (int e = 0; e < R::NP; ++e) {
+            const float4 z = keep[32 * e];
+            v1[2 * e] = z.x;
+            v1[2 * e + 1] = z.y;
+            v2[2 * e] = z.z;
+            v2[2 * e + 1] = z.w;
+          }
+          if (divide) {
+#pragma unroll 1
+            for (int e = 0; e < R::NP; ++e) {
+              float4* z = mine + (i * R::NP + e) * 32;
+              *z = make_float4(__fdiv_rn(z->x, s_new), __fdiv_rn(z->y, s_new), __fdiv_rn(z->z, s_new), __fdiv_rn(z->w, s_new));
             }
-          } else {
 #pragma unroll
             for (int e = 0; e < R::NP; ++e) {
               const float4 z = keep[32 * e];
-              y1[e] = make_float2(z.x, z.y);
-              y2[e] = make_float2(z.z, z.w);
+              v1[2 * e] = z.x;
+              v1[2 * e + 1] = z.y;
+              v2[2 * e] = z.z;
+              v2[2 * e + 1] = z.w;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < R::NE; ++e) {
+              v1[e] *= inv;
+              v2[e] *= inv;
             }
           }
-          if (pass == 0) {
-            // the largest first; where it is not finite, the finite ones one by one (the maximum
-            // passes NaN over, which the clamp's code keeps)
-            float big = 0.f;
 #pragma unroll
-            for (int e = 0; e < R::NP; ++e)
-              big = fmaxf(fmaxf(big, fmaxf(fabsf(y1[e].x), fabsf(y1[e].y))),
-                          fmaxf(fabsf(y2[e].x), fabsf(y2[e].y)));
-            if (big > 3.402823466e38f) {
-              big = 0.f;
-#pragma unroll
-              for (int e = 0; e < R::NP; ++e)
-                for (const float a : {y1[e].x, y1[e].y, y2[e].x, y2[e].y})
-                  if (fabsf(a) <= 3.402823466e38f) big = fmaxf(big, fabsf(a));
-            }
-            if (live) amax = fmaxf(amax, big);
-          } else if (live && on) {
-#pragma unroll
-            for (int c = 0; c < R::NC; ++c) {
-              const int at = piece_at<R>(c, j);
-              if (at >= p.half) continue;
-              float a[R::VEC], e2[R::VEC];
-#pragma unroll
-              for (int e = 0; e < R::VEC; ++e) {
-                const int z = c * R::VEC + e;
-                const float f1 = z & 1 ? y1[z / 2].y : y1[z / 2].x;
-                const float f2 = z & 1 ? y2[z / 2].y : y2[z / 2].x;
-                a[e] = divide ? __fdiv_rn(f1, s_new) : f1 * inv;
-                e2[e] = divide ? __fdiv_rn(f2, s_new) : f2 * inv;
-              }
-              unsigned char* y = pool + r * p.p_st + at;
-              store_codes<INT8, R::VEC>(y, a);
-              store_codes<INT8, R::VEC>(y + p.half, e2);
-            }
+          for (int c = 0; c < R::NC; ++c) {
+            const int at = piece_at<R>(c, j);
+            if (at >= p.half) continue;
+            unsigned char* y = pool + r * p.p_st + at;
+            store_codes<INT8, R::VEC>(y, v1 + c * R::VEC);
+            store_codes<INT8, R::VEC>(y + p.half, v2 + c * R::VEC);
           }
         }
       }
@@ -379,7 +398,7 @@ __global__ void __launch_bounds__(256, 2) append_quant_kernel(const AppendParams
           for (int c = 0; c < R::NC; ++c) {
             const int at = piece_at<R>(c, j);
             if (at >= p.half) continue;
-#pragma unroll
+#pragma unroll 1
             for (int hf = 0; hf < 2; ++hf) {
               unsigned char* y = pool + r * p.p_st + hf * p.half + at;
               float f[R::VEC];
