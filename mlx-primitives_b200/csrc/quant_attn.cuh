@@ -288,7 +288,7 @@ struct QaRing {
   static constexpr int KW = D / 16, VW = D / 32;   // words a lane holds of a K row, a V row
   static constexpr int KB = D == 32 ? 8 : 16, KP = 4 * KW / KB, VB = D / 8;
   static constexpr int kHalf = kQaTile * D, kTileBytes = 2 * kHalf;
-  static constexpr int kStages = D == 128 ? 3 : 4;
+  static constexpr int kStages = D == 128 ? 3 : 4;  // more gained nothing: 180 us at 3, 184 at 4
   // a warp's rows' scales and validity a stage, where the block size is not a multiple of 16
   static constexpr int kMeta = 32 * 20;
   static constexpr int kRing = kStages * kTileBytes;
@@ -608,24 +608,28 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
     const int ch1 = (int)min((long long)r.n, ch0 + (w.f_end - w.f));
     if (w.f == f_begin && threadIdx.x == 0) qa_write_info(p, w, r.n, hg, ch0);
     __syncthreads();  // the last unit's reads of the row tables and s_red are done
-    if (threadIdx.x < ROWS) {
-      const int row = r0 + threadIdx.x, i = row / p.G;
-      int lo = 0, hi = 0;
-      if (row < p.R && i < r.qlen) qa_row_range(p, r.ctx, r.qlen, i, lo, hi);
-      s_lo[threadIdx.x] = lo;
-      s_hi[threadIdx.x] = hi;
-      s_pos[threadIdx.x] = (int)(r.ctx - r.qlen + i);
-    }
-    if (p.alibi && threadIdx.x < HP * ROWS) {
-      const int hw = threadIdx.x / ROWS, row = r0 + threadIdx.x % ROWS;
-      s_slope[hw][threadIdx.x % ROWS] =
-          row < p.R ? __ldg(p.alibi + (hg * HP + hw) * p.G + row % p.G) * 1.4426950408889634f : 0.f;
-    }
-    __syncthreads();
     const int hk = hg * HP + hp;
     uint32_t qf[SPLIT ? 2 : 1][NT][D / 16][2];
     float qs[NT][2];
-    qa_load_q<T, D, NT, SPLIT>(p, b, r0, hk, g, c, qf, qs);
+    // The rows' tables and this warp's queries: called by every warp once its first tiles are on
+    // their way.
+    auto set_up = [&] {
+      if (threadIdx.x < ROWS) {
+        const int row = r0 + threadIdx.x, i = row / p.G;
+        int lo = 0, hi = 0;
+        if (row < p.R && i < r.qlen) qa_row_range(p, r.ctx, r.qlen, i, lo, hi);
+        s_lo[threadIdx.x] = lo;
+        s_hi[threadIdx.x] = hi;
+        s_pos[threadIdx.x] = (int)(r.ctx - r.qlen + i);
+      }
+      if (p.alibi && threadIdx.x < HP * ROWS) {
+        const int hw = threadIdx.x / ROWS, row = r0 + threadIdx.x % ROWS;
+        s_slope[hw][threadIdx.x % ROWS] =
+            row < p.R ? __ldg(p.alibi + (hg * HP + hw) * p.G + row % p.G) * 1.4426950408889634f : 0.f;
+      }
+      __syncthreads();
+      qa_load_q<T, D, NT, SPLIT>(p, b, r0, hk, g, c, qf, qs);
+    };
     QaState<D, NT> st;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -664,13 +668,12 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
             x.id = got;
             x.ks = __ldg(p.k_scales + got * p.sc_sb + head_sc);
             x.vs = __ldg(p.v_scales + got * p.sc_sb + head_sc);
-            x.lv = qa_log_scale(x.vs);
           }
         }
         x.there = __ballot_sync(0xffffffffu, x.id >= 0);
         return x;
       };
-      Batch cur = batch(0), next = batch(32);
+      Batch cur = batch(0), next = batch(32);  // lv: once the scale is here and is needed
       int base = 0;  // first tile of `cur`
       int inflight = 0;
       stage_in = stage_out;
@@ -693,6 +696,8 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
       __syncwarp();
       int ahead = 0;             // tiles issued so far
       for (; ahead < Q::kStages; ++ahead) issue(ahead);
+      set_up();
+      cur.lv = qa_log_scale(cur.vs);
       bool ok = true;
       for (int i = 0; i < tiles; ++i) {
         if (cur.there >> (i & 31) & 1u) {
@@ -721,6 +726,7 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
         if ((i & 31) == 31) {
           base += 32;
           cur = next;
+          cur.lv = qa_log_scale(cur.vs);
           next = batch(base + 32);
           while (inflight < Q::kStages && ahead < tiles && ahead - base < 64) issue(ahead++);
         }
@@ -734,6 +740,7 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
       }
     } else {
       // Any block size: every lane copies the pieces that it reads itself, with cp.async.
+      set_up();
       const unsigned char* kl = p.k_pool + hk * p.p_sh + Q::KB * c;
       const unsigned char* vl = p.v_pool + hk * p.p_sh + Q::VB * qa_piece<D>(g);
       auto locate = [&](int key, long long& off) {
