@@ -3,7 +3,8 @@
     python mlx-primitives_b200/csrc/build.py [--force] [--debug]
 
 The library lands next to the Python package (mlx_primitives/libmlxp_attn.so) so that it
-travels with the source tree; the Python shim loads it from there (or from $MLXP_LIB).
+travels with the source tree; the Python shim loads it from there (or from $MLXP_LIB).  Beside it
+goes _host.so, the C++ half of the shim (host_calls.cpp, built with g++ against torch's headers).
 """
 
 from __future__ import annotations
@@ -14,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
@@ -22,7 +24,9 @@ INCLUDE = PKG_ROOT.parent / "include"
 OUT = PKG_ROOT / "mlx_primitives" / "libmlxp_attn.so"
 SOURCES = [CSRC / "mlxp_attn.cu", CSRC / "mlxp_cache.cu", CSRC / "mlxp_quant.cu",
            CSRC / "mlxp_quant_rows.cu"]
-DEPS = SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [INCLUDE / "mlxp_attn.h"]
+HOST_SOURCE = CSRC / "host_calls.cpp"
+HOST_OUT = PKG_ROOT / "mlx_primitives" / "_host.so"
+DEPS = SOURCES + [HOST_SOURCE] + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [INCLUDE / "mlxp_attn.h"]
 OBJ = CSRC / "_build"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -51,10 +55,25 @@ def commands(debug: bool = False, verbose_ptxas: bool = False) -> tuple[list[lis
     return compiles, link
 
 
+def host_command() -> list[str]:
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-isystem", str(root / "include"),
+            "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+            "-isystem", sysconfig.get_paths()["include"],
+            "-isystem", str(Path(nvcc_path()).resolve().parent.parent / "include"),
+            "-o", str(HOST_OUT), str(HOST_SOURCE),
+            "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+            f"-Wl,-rpath,{root / 'lib'}"]
+
+
 def up_to_date() -> bool:
-    if not OUT.exists():
+    if not OUT.exists() or not HOST_OUT.exists():
         return False
-    t = OUT.stat().st_mtime
+    t = min(OUT.stat().st_mtime, HOST_OUT.stat().st_mtime)
     return all(d.stat().st_mtime <= t for d in DEPS if d.exists())
 
 
@@ -67,12 +86,12 @@ def build(force: bool = False, debug: bool = False, verbose_ptxas: bool = False)
     def run(cmd):
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
-            raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+            raise RuntimeError("compiler failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
         if verbose_ptxas:
             sys.stderr.write(res.stderr)
 
     with concurrent.futures.ThreadPoolExecutor() as pool:
-        list(pool.map(run, compiles))
+        list(pool.map(run, [*compiles, host_command()]))
     run(link)
     return OUT
 

@@ -1,0 +1,359 @@
+// host_calls.cpp — the short way from Python to the cache operators' C entry points.
+//
+// A decode step's kernels take a few microseconds; checking a dozen tensors and packing their
+// addresses and strides in Python took 10 to 14.  These functions do the same in C++ for calls
+// whose tensors can be used as they are (dtypes, devices, strides, no gradients), and return None
+// for every other call, which the Python entry points then take themselves: the checks and their
+// messages, conversions and copies live there only.  A nonzero status comes back as an int.
+//
+// The library's functions are handed over by address (bind), so that this module and ctypes share
+// one copy of it, wherever $MLXP_LIB says it is.
+
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+
+#include "../../include/mlxp_attn.h"
+
+namespace {
+
+int (*g_norm_rope)(const mlxp_qk_norm_rope_args*) = nullptr;
+int (*g_append)(const mlxp_paged_append_args*) = nullptr;
+int (*g_attn)(const mlxp_quant_paged_attn_args*) = nullptr;
+size_t (*g_attn_ws)(const mlxp_quant_paged_attn_args*) = nullptr;
+
+// One argument: a tensor, None, or something that this path does not take.
+struct Arg {
+  const at::Tensor* t = nullptr;
+  bool ok = true;
+  explicit Arg(PyObject* o) {
+    if (o == Py_None) return;
+    if (!THPVariable_CheckExact(o)) {
+      ok = false;
+      return;
+    }
+    t = &THPVariable_Unpack(o);
+  }
+  explicit operator bool() const { return t != nullptr; }
+  const at::Tensor* operator->() const { return t; }
+  void* data() const { return t ? t->data_ptr() : nullptr; }
+};
+
+int code_of(at::ScalarType s) {
+  switch (s) {
+    case at::kFloat: return MLXP_DTYPE_FP32;
+    case at::kBFloat16: return MLXP_DTYPE_BF16;
+    case at::kHalf: return MLXP_DTYPE_FP16;
+    default: return -1;
+  }
+}
+
+int cache_code_of(at::ScalarType s) {
+  if (s == at::kFloat8_e4m3fn) return MLXP_DTYPE_E4M3;
+  if (s == at::kChar) return MLXP_DTYPE_INT8;
+  return -1;
+}
+
+bool on(const Arg& a, int64_t dev) { return a->is_cuda() && a->get_device() == dev; }
+bool wants_grad(const Arg& a) { return a && a->requires_grad(); }
+
+// (batch, seq, heads, dim) tensor with unit dim stride.
+bool rows(const Arg& a, int64_t dev) { return a && a->dim() == 4 && on(a, dev) && a->stride(3) == 1; }
+
+bool ints(const Arg& a, int64_t dev, int64_t n) {
+  return a->scalar_type() == at::kInt && on(a, dev) && a->dim() == 1 && a->size(0) == n && a->is_contiguous();
+}
+
+bool table(const Arg& a, int64_t dev, int64_t half) {
+  return a->scalar_type() == at::kFloat && on(a, dev) && a->dim() == 2 && a->size(1) == half && a->is_contiguous();
+}
+
+bool weight(const Arg& a, int64_t dev, int64_t D) {
+  return code_of(a->scalar_type()) >= 0 && on(a, dev) && a->dim() == 1 && a->size(0) == D && a->is_contiguous();
+}
+
+void seq_strides(int64_t (&to)[3], const at::Tensor& t) {
+  to[0] = t.stride(0);
+  to[1] = t.stride(2);
+  to[2] = t.stride(1);
+}
+
+void* stream_of(int64_t dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
+
+PyObject* none() { Py_RETURN_NONE; }
+
+// Pools of either operator: same shape, strides and dtype, unit dim stride.
+bool pools(const Arg& k, const Arg& v, int64_t dev) {
+  return rows(k, dev) && rows(v, dev) && k->sizes() == v->sizes() && k->strides() == v->strides() &&
+         k->scalar_type() == v->scalar_type();
+}
+
+bool scales(const Arg& k, const Arg& v, int64_t dev, int64_t blocks, int64_t heads) {
+  for (const Arg* s : {&k, &v})
+    if (!*s || (*s)->scalar_type() != at::kFloat || !on(*s, dev) || (*s)->dim() != 2 || (*s)->size(0) != blocks ||
+        (*s)->size(1) != heads || !(*s)->is_contiguous())
+      return false;
+  return true;
+}
+
+// Every function: C++ exceptions become Python's.
+template <typename F>
+PyObject* guarded(F&& f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// norm_rope(q, k, q_weight, k_weight, cos, sin, positions, offset, k_offset, eps) -> (q, k)
+PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 10 || !g_norm_rope || !PyLong_CheckExact(a[7]) || !PyLong_CheckExact(a[8]) || !PyFloat_CheckExact(a[9]))
+    return none();
+  return guarded([&]() -> PyObject* {
+    const Arg q(a[0]), k(a[1]), qw(a[2]), kw(a[3]), c(a[4]), s(a[5]), pos(a[6]);
+    if (!q.ok || !k.ok || !qw.ok || !kw.ok || !c.ok || !s.ok || !pos.ok || !q || !k || !q->is_cuda()) return none();
+    const int64_t dev = q->get_device();
+    const int code = code_of(q->scalar_type());
+    if (code < 0 || !rows(q, dev) || !rows(k, dev) || k->scalar_type() != q->scalar_type() ||
+        dev != c10::cuda::current_device())
+      return none();
+    const int64_t B = q->size(0), D = q->size(3);
+    if (k->size(0) != B || k->size(3) != D || D < 2 || D % 2 || bool(qw) != bool(kw) || bool(c) != bool(s)) return none();
+    if (qw && !(weight(qw, dev, D) && weight(kw, dev, D))) return none();
+    if (c && !(table(c, dev, D / 2) && table(s, dev, D / 2) && c->size(0) == s->size(0))) return none();
+    if (pos && (pos->scalar_type() != at::kInt || !on(pos, dev) || pos->dim() != 2 || pos->size(0) != B ||
+                pos->size(1) != q->size(1) || q->size(1) != k->size(1)))
+      return none();
+    if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(qw) || wants_grad(kw))) return none();
+    at::Tensor qo = at::empty_like(*q.t), ko = at::empty_like(*k.t);
+    mlxp_qk_norm_rope_args x{};
+    x.size = sizeof(x);
+    x.q = q.data();
+    x.k = k.data();
+    x.q_out = qo.data_ptr();
+    x.k_out = ko.data_ptr();
+    x.q_weight = qw.data();
+    x.k_weight = kw.data();
+    x.cos_cache = static_cast<const float*>(c.data());
+    x.sin_cache = static_cast<const float*>(s.data());
+    x.positions = static_cast<const int32_t*>(pos.data());
+    x.dtype = code;
+    x.q_weight_dtype = qw ? code_of(qw->scalar_type()) : 0;
+    x.k_weight_dtype = kw ? code_of(kw->scalar_type()) : 0;
+    x.B = B;
+    x.Sq = q->size(1);
+    x.Sk = k->size(1);
+    x.Hq = q->size(2);
+    x.Hk = k->size(2);
+    x.D = D;
+    x.n_pos = c ? c->size(0) : 0;
+    x.q_offset = PyLong_AsLongLong(a[7]);
+    x.k_offset = PyLong_AsLongLong(a[8]);
+    if (PyErr_Occurred()) return nullptr;
+    if (pos) {
+      x.pos_strides[0] = pos->stride(0);
+      x.pos_strides[1] = pos->stride(1);
+    }
+    seq_strides(x.q_strides, *q.t);
+    seq_strides(x.k_strides, *k.t);
+    seq_strides(x.q_out_strides, qo);
+    seq_strides(x.k_out_strides, ko);
+    x.eps = PyFloat_AS_DOUBLE(a[9]);
+    x.stream = stream_of(dev);
+    if (const int rc = g_norm_rope(&x)) return PyLong_FromLong(rc);
+    PyObject* out = PyTuple_New(2);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(qo)));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(ko)));
+    return out;
+  });
+}
+
+// append(k, v, k_pool, v_pool, block_tables, context_lens, new_lens, q, cos, sin, q_weight, k_weight,
+//        k_scales, v_scales, eps) -> q, or True without one
+PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 15 || !g_append || !PyFloat_CheckExact(a[14])) return none();
+  return guarded([&]() -> PyObject* {
+    const Arg k(a[0]), v(a[1]), kp(a[2]), vp(a[3]), bt(a[4]), ctx(a[5]), fresh(a[6]), q(a[7]), c(a[8]), s(a[9]),
+        qw(a[10]), kw(a[11]), ks(a[12]), vs(a[13]);
+    for (const Arg* x : {&k, &v, &kp, &vp, &bt, &ctx, &fresh, &q, &c, &s, &qw, &kw, &ks, &vs})
+      if (!x->ok) return none();
+    if (!k || !v || !kp || !vp || !bt || !ctx || !k->is_cuda()) return none();
+    const int64_t dev = k->get_device();
+    const int code = code_of(k->scalar_type());
+    if (code < 0 || dev != c10::cuda::current_device() || !rows(k, dev) || !rows(v, dev) ||
+        k->sizes() != v->sizes() || v->scalar_type() != k->scalar_type() || !pools(kp, vp, dev) || !kp->is_contiguous())
+      return none();
+    const int64_t B = k->size(0), S = k->size(1), Hk = k->size(2), D = k->size(3);
+    if (kp->size(2) != Hk || kp->size(3) != D || D < 2 || D % 2) return none();
+    int cache = cache_code_of(kp->scalar_type());
+    if (cache >= 0) {
+      if (!scales(ks, vs, dev, kp->size(0), Hk)) return none();
+    } else {
+      if (ks || vs || kp->scalar_type() != k->scalar_type()) return none();
+      cache = code;
+    }
+    if (bt->scalar_type() != at::kInt || !on(bt, dev) || bt->dim() != 2 || bt->size(0) != B || !bt->is_contiguous() ||
+        !ints(ctx, dev, B) || (fresh && !ints(fresh, dev, B)))
+      return none();
+    const int64_t mb = bt->size(1), block = kp->size(1);
+    if (q && (!rows(q, dev) || q->size(0) != B || q->size(1) != S || q->size(3) != D ||
+              q->scalar_type() != k->scalar_type()))
+      return none();
+    if ((qw && (!q || !weight(qw, dev, D))) || (kw && !weight(kw, dev, D)) || bool(c) != bool(s)) return none();
+    if (c && !(table(c, dev, D / 2) && table(s, dev, D / 2) && c->size(0) == s->size(0) && c->size(0) >= mb * block))
+      return none();
+    if (at::GradMode::is_enabled() && (wants_grad(k) || wants_grad(v) || wants_grad(q) || wants_grad(qw) || wants_grad(kw)))
+      return none();
+    mlxp_paged_append_args x{};
+    x.size = sizeof(x);
+    at::Tensor qo;
+    if (q) {
+      qo = at::empty_like(*q.t);
+      x.q = q.data();
+      x.q_out = qo.data_ptr();
+      x.Hq = q->size(2);
+      seq_strides(x.q_strides, *q.t);
+      seq_strides(x.q_out_strides, qo);
+    }
+    x.k = k.data();
+    x.v = v.data();
+    x.k_pool = kp.data();
+    x.v_pool = vp.data();
+    x.k_scales = static_cast<float*>(ks.data());
+    x.v_scales = static_cast<float*>(vs.data());
+    x.block_tables = static_cast<const int32_t*>(bt.data());
+    x.context_lens = static_cast<const int32_t*>(ctx.data());
+    x.new_lens = static_cast<const int32_t*>(fresh.data());
+    x.q_weight = qw.data();
+    x.k_weight = kw.data();
+    x.cos_cache = static_cast<const float*>(c.data());
+    x.sin_cache = static_cast<const float*>(s.data());
+    x.dtype = code;
+    x.cache_dtype = cache;
+    x.q_weight_dtype = qw ? code_of(qw->scalar_type()) : 0;
+    x.k_weight_dtype = kw ? code_of(kw->scalar_type()) : 0;
+    x.B = B;
+    x.S = S;
+    x.Hk = Hk;
+    x.D = D;
+    x.num_blocks = kp->size(0);
+    x.block_size = block;
+    x.max_blocks = mb;
+    x.bt_stride = bt->stride(0);
+    x.n_pos = c ? c->size(0) : 0;
+    seq_strides(x.k_strides, *k.t);
+    seq_strides(x.v_strides, *v.t);
+    for (int i = 0; i < 3; ++i) x.pool_strides[i] = kp->stride(i);
+    if (ks)
+      for (int i = 0; i < 2; ++i) x.scale_strides[i] = ks->stride(i);
+    x.eps = PyFloat_AS_DOUBLE(a[14]);
+    x.stream = stream_of(dev);
+    if (const int rc = g_append(&x)) return PyLong_FromLong(rc);
+    if (!q) Py_RETURN_TRUE;
+    return THPVariable_Wrap(std::move(qo));
+  });
+}
+
+// attend(q, k_pool, v_pool, k_scales, v_scales, block_tables, context_lens, query_lens, scale or None, causal,
+//        window (-1: none)) -> o
+PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 11 || !g_attn || !(a[8] == Py_None || PyFloat_CheckExact(a[8])) || !PyLong_Check(a[9]) || !PyLong_CheckExact(a[10])) return none();
+  return guarded([&]() -> PyObject* {
+    const Arg q(a[0]), kp(a[1]), vp(a[2]), ks(a[3]), vs(a[4]), bt(a[5]), ctx(a[6]), lens(a[7]);
+    for (const Arg* x : {&q, &kp, &vp, &ks, &vs, &bt, &ctx, &lens})
+      if (!x->ok) return none();
+    if (!q || !kp || !vp || !bt || !ctx || !q->is_cuda()) return none();
+    const int64_t dev = q->get_device();
+    const int code = code_of(q->scalar_type());
+    if (code < 0 || dev != c10::cuda::current_device() || !rows(q, dev) || !pools(kp, vp, dev)) return none();
+    const int64_t B = q->size(0), D = q->size(3), H = q->size(2), Hk = kp->size(2), es = q->element_size();
+    const int cache = cache_code_of(kp->scalar_type());
+    if (cache < 0 || kp->size(3) != D || (D != 32 && D != 64 && D != 128) || Hk < 1 || H < 1 || H % Hk ||
+        !scales(ks, vs, dev, kp->size(0), Hk))
+      return none();
+    if ((reinterpret_cast<uintptr_t>(q.data()) | q->stride(0) * es | q->stride(1) * es | q->stride(2) * es) & 15)
+      return none();
+    if (bt->scalar_type() != at::kInt || !on(bt, dev) || bt->dim() != 2 || bt->size(0) != B || !bt->is_contiguous() ||
+        !ints(ctx, dev, B) || (lens && !ints(lens, dev, B)))
+      return none();
+    if (at::GradMode::is_enabled() && wants_grad(q)) return none();
+    at::Tensor o = at::empty_like(*q.t);
+    mlxp_quant_paged_attn_args x{};
+    x.size = sizeof(x);
+    x.q = q.data();
+    x.o = o.data_ptr();
+    x.k_pool = kp.data();
+    x.v_pool = vp.data();
+    x.k_scales = static_cast<const float*>(ks.data());
+    x.v_scales = static_cast<const float*>(vs.data());
+    x.block_tables = static_cast<const int32_t*>(bt.data());
+    x.context_lens = static_cast<const int32_t*>(ctx.data());
+    x.query_lens = static_cast<const int32_t*>(lens.data());
+    x.dtype = code;
+    x.cache_dtype = cache;
+    x.B = B;
+    x.Sq = q->size(1);
+    x.H = H;
+    x.kv_heads = Hk;
+    x.D = D;
+    x.num_blocks = kp->size(0);
+    x.block_size = kp->size(1);
+    x.max_blocks = bt->size(1);
+    x.bt_stride = bt->stride(0);
+    x.causal = PyObject_IsTrue(a[9]);
+    x.window = PyLong_AsLongLong(a[10]);
+    if (PyErr_Occurred()) return nullptr;
+    seq_strides(x.q_strides, *q.t);
+    seq_strides(x.o_strides, o);
+    for (int i = 0; i < 3; ++i) x.pool_strides[i] = kp->stride(i);
+    for (int i = 0; i < 2; ++i) x.scale_strides[i] = ks->stride(i);
+    x.scale = a[8] == Py_None ? 1.0 / std::sqrt((double)D) : PyFloat_AS_DOUBLE(a[8]);
+    x.stream = stream_of(dev);
+    x.ws_bytes = g_attn_ws(&x);
+    at::Tensor ws = at::empty({(int64_t)x.ws_bytes}, q->options().dtype(at::kByte));
+    x.workspace = ws.data_ptr();
+    if (const int rc = g_attn(&x)) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(std::move(o));
+  });
+}
+
+// bind(norm_rope, append, attend, attend workspace): the library's functions, as addresses
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 4) {
+    PyErr_SetString(PyExc_TypeError, "bind takes four addresses");
+    return nullptr;
+  }
+  void* p[4];
+  for (int i = 0; i < 4; ++i) {
+    p[i] = PyLong_AsVoidPtr(a[i]);
+    if (PyErr_Occurred()) return nullptr;
+  }
+  g_norm_rope = reinterpret_cast<int (*)(const mlxp_qk_norm_rope_args*)>(p[0]);
+  g_append = reinterpret_cast<int (*)(const mlxp_paged_append_args*)>(p[1]);
+  g_attn = reinterpret_cast<int (*)(const mlxp_quant_paged_attn_args*)>(p[2]);
+  g_attn_ws = reinterpret_cast<size_t (*)(const mlxp_quant_paged_attn_args*)>(p[3]);
+  Py_RETURN_NONE;
+}
+
+PyMethodDef g_methods[] = {
+    {"norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(norm_rope)), METH_FASTCALL, nullptr},
+    {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(append)), METH_FASTCALL, nullptr},
+    {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attend)), METH_FASTCALL, nullptr},
+    {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", "Short calls of the cache operators.", -1, g_methods,
+                        nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__host() { return PyModule_Create(&g_module); }

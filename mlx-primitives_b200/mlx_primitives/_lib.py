@@ -144,6 +144,26 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_calls = None
+
+
+def calls():
+    """The _host module (csrc/host_calls.cpp): the cache operators' short calls, on this library."""
+    global _calls
+    if _calls is None:
+        L = lib()
+        try:
+            from . import _host
+        except ImportError as e:
+            raise ImportError("mlx_primitives/_host.so is missing or does not match this torch; build it "
+                              "with `python mlx-primitives_b200/csrc/build.py`") from e
+        _host.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            L.mlxp_qk_norm_rope, L.mlxp_paged_append, L.mlxp_quant_paged_attn,
+            L.mlxp_quant_paged_attn_workspace_size)))
+        _calls = _host
+    return _calls
+
+
 def last_error() -> str:
     msg = lib().mlxp_last_error()
     return msg.decode() if msg else ""

@@ -106,6 +106,12 @@ def paged_append(
     it to.  A block that receives tokens must belong to one sequence (full blocks may be shared):
     the order of two writers of a block is not defined.  Not differentiable.
     """
+    out = _lib.calls().append(k, v, k_pool, v_pool, block_tables, context_lens, new_lens, q, cos_cache,
+                              sin_cache, q_weight, k_weight, k_scales, v_scales, eps)
+    if out is not None:  # else: not a call that can be made as it is
+        if type(out) is int:
+            _lib.check(out, "mlxp_paged_append")
+        return None if out is True else out
     shape = k.shape
     if len(shape) != 4 or v.shape != shape:
         raise ValueError("k and v must both be (batch, seq, kv_heads, head_dim), got "

@@ -59,6 +59,14 @@ def quantized_paged_attention(
     ALiBi adds slope[h] * (key position - query position).  Returns q's shape and dtype.  Not
     differentiable.
     """
+    if alibi_slopes is None and (window_size is None or window_size >= 0):
+        out = _lib.calls().attend(q, k_pool, v_pool, k_scales, v_scales, block_tables, context_lens,
+                                  query_lens, scale, causal,
+                                  -1 if window_size is None else window_size)
+        if out is not None:  # else: not a call that can be made as it is
+            if type(out) is int:
+                _lib.check(out, "mlxp_quant_paged_attn")
+            return out
     shape = q.shape
     if len(shape) != 4:
         raise ValueError(f"q must be (batch, seq_q, num_heads, head_dim), got {tuple(q.shape)}")

@@ -176,6 +176,12 @@ def qk_norm_rope(
     no gradient; one past the tables gives a row of NaN (it is read on the device, where it
     cannot be refused).  head_dim is even and at most 256.
     """
+    out = _lib.calls().norm_rope(q, k, q_weight, k_weight, cos_cache, sin_cache, positions, offset,
+                                 offset if k_offset is None else k_offset, eps)
+    if out is not None:  # else: not a call that can be made as it is
+        if type(out) is int:
+            _lib.check(out, "mlxp_qk_norm_rope")
+        return out
     if not _quick_ok(q, k, q_weight, k_weight, cos_cache, sin_cache, positions):
         _refuse(q, k, q_weight, k_weight, cos_cache, sin_cache, positions)
     needs = torch.is_grad_enabled() and (

@@ -185,3 +185,21 @@ def test_quantized_paged_attention_refusals():
         f(q, pool, pool, sc, sc, bt, ctx, alibi_slopes=_t(3))
     with pytest.raises(NotImplementedError, match="differentiable"):
         f(q.requires_grad_(True), pool, pool, sc, sc, bt, ctx)
+
+
+def test_short_calls_leave_what_they_do_not_take_to_python():
+    """The C++ half of the shim answers None (take the long way) to anything but device tensors
+    that can be used as they are, and never raises for them."""
+    from mlx_primitives import _lib
+    calls = _lib.calls()
+    q, w, cs = _t(1, 4, 2, 8), _t(8), _t(4, 4)
+    assert calls.norm_rope(q, q, w, w, cs, cs, None, 0, 0, 1e-6) is None           # host tensors
+    assert calls.norm_rope(q, 3, w, w, cs, cs, None, 0, 0, 1e-6) is None           # not a tensor
+    assert calls.norm_rope(q, q, w, w, cs, cs, None, 0, 0, 1) is None              # eps not a float
+    assert calls.norm_rope(q) is None
+    pool, i = _t(3, 16, 2, 8), _t(1, dtype=torch.int32)
+    assert calls.append(q, q, pool, pool, _t(1, 1, dtype=torch.int32), i, None, None, None, None, None,
+                        None, None, None, 1e-6) is None
+    assert calls.append(*[None] * 14, 1e-6) is None
+    assert calls.attend(q, pool, pool, None, None, _t(1, 1, dtype=torch.int32), i, None, None, True, -1) is None
+    assert calls.attend(*[None] * 9, True, -1) is None
