@@ -2,8 +2,8 @@
 //
 // A decode step's kernels take a few microseconds; checking a dozen tensors and packing their
 // addresses and strides in Python took 10 to 14.  These functions do the same in C++ for calls
-// whose tensors can be used as they are (dtypes, devices, strides, no gradients), and return None
-// for every other call, which the Python entry points then take themselves: the checks and their
+// whose tensors can be used as they are (dtypes, devices, strides), and return None for every
+// other call, which the Python entry points then take themselves: the checks and their
 // messages, conversions and copies live there only.  A nonzero status comes back as an int.
 //
 // The library's functions are handed over by address (bind), so that this module and ctypes share
@@ -15,15 +15,22 @@
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <optional>
+#include <stdexcept>
+#include <string>
 
 #include "../../include/mlxp_attn.h"
 
 namespace {
 
 int (*g_norm_rope)(const mlxp_qk_norm_rope_args*) = nullptr;
+int (*g_norm_rope_bwd)(const mlxp_qk_norm_rope_args*) = nullptr;
+size_t (*g_norm_rope_ws)(int64_t) = nullptr;
 int (*g_append)(const mlxp_paged_append_args*) = nullptr;
 int (*g_attn)(const mlxp_quant_paged_attn_args*) = nullptr;
 size_t (*g_attn_ws)(const mlxp_quant_paged_attn_args*) = nullptr;
@@ -113,6 +120,136 @@ PyObject* guarded(F&& f) {
   }
 }
 
+// ---- norm + rotation, with its gradient -------------------------------------------------------
+
+struct Status {  // of a launch inside the autograd function
+  int rc;
+};
+
+// What the forward and the backward have in common; undefined tensors are not there.
+mlxp_qk_norm_rope_args norm_rope_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw,
+                                      const at::Tensor& kw, const at::Tensor& c, const at::Tensor& s,
+                                      const at::Tensor& pos, int64_t offset, int64_t k_offset, double eps) {
+  mlxp_qk_norm_rope_args x{};
+  x.size = sizeof(x);
+  x.q = q.data_ptr();
+  x.k = k.data_ptr();
+  x.dtype = code_of(q.scalar_type());
+  x.B = q.size(0);
+  x.Sq = q.size(1);
+  x.Sk = k.size(1);
+  x.Hq = q.size(2);
+  x.Hk = k.size(2);
+  x.D = q.size(3);
+  if (qw.defined()) {
+    x.q_weight = qw.data_ptr();
+    x.k_weight = kw.data_ptr();
+    x.q_weight_dtype = code_of(qw.scalar_type());
+    x.k_weight_dtype = code_of(kw.scalar_type());
+  }
+  if (c.defined()) {
+    x.cos_cache = c.data_ptr<float>();
+    x.sin_cache = s.data_ptr<float>();
+    x.n_pos = c.size(0);
+  }
+  if (pos.defined()) {
+    x.positions = pos.data_ptr<int32_t>();
+    x.pos_strides[0] = pos.stride(0);
+    x.pos_strides[1] = pos.stride(1);
+  }
+  x.q_offset = offset;
+  x.k_offset = k_offset;
+  seq_strides(x.q_strides, q);
+  seq_strides(x.k_strides, k);
+  x.eps = eps;
+  x.stream = stream_of(q.get_device());
+  return x;
+}
+
+void set_outputs(mlxp_qk_norm_rope_args& x, const at::Tensor& qo, const at::Tensor& ko) {
+  if (qo.defined()) {
+    x.q_out = qo.data_ptr();
+    seq_strides(x.q_out_strides, qo);
+  }
+  if (ko.defined()) {
+    x.k_out = ko.data_ptr();
+    seq_strides(x.k_out_strides, ko);
+  }
+}
+
+using torch::autograd::variable_list;
+
+struct NormRopeFn : torch::autograd::Function<NormRopeFn> {
+  using Maybe = std::optional<at::Tensor>;
+  static variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
+                               const Maybe& qw_, const Maybe& kw_, const Maybe& c_, const Maybe& s_, const Maybe& pos_,
+                               int64_t offset, int64_t k_offset, double eps) {
+    const at::Tensor no;
+    const at::Tensor &qw = qw_ ? *qw_ : no, &kw = kw_ ? *kw_ : no, &c = c_ ? *c_ : no, &s = s_ ? *s_ : no,
+                     &pos = pos_ ? *pos_ : no;
+    at::Tensor qo = at::empty_like(q), ko = at::empty_like(k);
+    auto x = norm_rope_args(q, k, qw, kw, c, s, pos, offset, k_offset, eps);
+    set_outputs(x, qo, ko);
+    if (const int rc = g_norm_rope(&x)) throw Status{rc};
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({q, k, qw, kw, c, s, pos});
+    ctx->saved_data["offset"] = offset;
+    ctx->saved_data["k_offset"] = k_offset;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["dqw"] = qw.defined() && qw.requires_grad();
+    ctx->saved_data["dkw"] = kw.defined() && kw.requires_grad();
+    return {qo, ko};
+  }
+
+  static variable_list backward(torch::autograd::AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &k = saved[1], &qw = saved[2], &kw = saved[3];
+    for (at::Tensor& t : g)
+      if (t.defined() && t.stride(3) != 1) t = t.contiguous();
+    variable_list out(10);
+    {
+      at::NoGradGuard no_grad;
+      if (g[0].defined()) out[0] = at::empty_like(q);
+      if (g[1].defined()) out[1] = at::empty_like(k);
+      if (ctx->saved_data["dqw"].toBool()) out[2] = at::empty_like(qw);
+      if (ctx->saved_data["dkw"].toBool()) out[3] = at::empty_like(kw);
+      auto x = norm_rope_args(q, k, qw, kw, saved[4], saved[5], saved[6], ctx->saved_data["offset"].toInt(),
+                              ctx->saved_data["k_offset"].toInt(), ctx->saved_data["eps"].toDouble());
+      set_outputs(x, out[0], out[1]);
+      if (g[0].defined()) {
+        x.gq = g[0].data_ptr();
+        seq_strides(x.gq_strides, g[0]);
+      }
+      if (g[1].defined()) {
+        x.gk = g[1].data_ptr();
+        seq_strides(x.gk_strides, g[1]);
+      }
+      at::Tensor ws;
+      if (out[2].defined() || out[3].defined()) {
+        if (out[2].defined()) x.dq_weight = out[2].data_ptr();
+        if (out[3].defined()) x.dk_weight = out[3].data_ptr();
+        x.ws_bytes = g_norm_rope_ws(x.D);
+        ws = at::empty({(int64_t)x.ws_bytes}, q.options().dtype(at::kByte));
+        x.workspace = ws.data_ptr();
+      }
+      if (const int rc = g_norm_rope_bwd(&x))
+        throw std::runtime_error("mlxp_qk_norm_rope_bwd failed with status " + std::to_string(rc));
+    }
+    if (at::GradMode::is_enabled()) {  // gradients of these are refused when they are asked for
+      variable_list there;
+      for (const at::Tensor& t : out)
+        if (t.defined()) there.push_back(t.detach().requires_grad_(true));
+      auto refuse = std::make_shared<torch::autograd::DelayedError>(
+          "qk_norm_rope has no second derivative", (int64_t)there.size());
+      there = (*refuse)(std::move(there));
+      size_t i = 0;
+      for (at::Tensor& t : out)
+        if (t.defined()) t = there[i++];
+    }
+    return out;
+  }
+};
+
 // norm_rope(q, k, q_weight, k_weight, cos, sin, positions, offset, k_offset, eps) -> (q, k)
 PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 10 || !g_norm_rope || !PyLong_CheckExact(a[7]) || !PyLong_CheckExact(a[8]) || !PyFloat_CheckExact(a[9]))
@@ -121,54 +258,41 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Arg q(a[0]), k(a[1]), qw(a[2]), kw(a[3]), c(a[4]), s(a[5]), pos(a[6]);
     if (!q.ok || !k.ok || !qw.ok || !kw.ok || !c.ok || !s.ok || !pos.ok || !q || !k || !q->is_cuda()) return none();
     const int64_t dev = q->get_device();
-    const int code = code_of(q->scalar_type());
-    if (code < 0 || !rows(q, dev) || !rows(k, dev) || k->scalar_type() != q->scalar_type() ||
+    if (code_of(q->scalar_type()) < 0 || !rows(q, dev) || !rows(k, dev) || k->scalar_type() != q->scalar_type() ||
         dev != c10::cuda::current_device())
       return none();
     const int64_t B = q->size(0), D = q->size(3);
     if (k->size(0) != B || k->size(3) != D || D < 2 || D % 2 || bool(qw) != bool(kw) || bool(c) != bool(s)) return none();
     if (qw && !(weight(qw, dev, D) && weight(kw, dev, D))) return none();
     if (c && !(table(c, dev, D / 2) && table(s, dev, D / 2) && c->size(0) == s->size(0))) return none();
+    if (wants_grad(c) || wants_grad(s)) return none();
     if (pos && (pos->scalar_type() != at::kInt || !on(pos, dev) || pos->dim() != 2 || pos->size(0) != B ||
                 pos->size(1) != q->size(1) || q->size(1) != k->size(1)))
       return none();
-    if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(qw) || wants_grad(kw))) return none();
-    at::Tensor qo = at::empty_like(*q.t), ko = at::empty_like(*k.t);
-    mlxp_qk_norm_rope_args x{};
-    x.size = sizeof(x);
-    x.q = q.data();
-    x.k = k.data();
-    x.q_out = qo.data_ptr();
-    x.k_out = ko.data_ptr();
-    x.q_weight = qw.data();
-    x.k_weight = kw.data();
-    x.cos_cache = static_cast<const float*>(c.data());
-    x.sin_cache = static_cast<const float*>(s.data());
-    x.positions = static_cast<const int32_t*>(pos.data());
-    x.dtype = code;
-    x.q_weight_dtype = qw ? code_of(qw->scalar_type()) : 0;
-    x.k_weight_dtype = kw ? code_of(kw->scalar_type()) : 0;
-    x.B = B;
-    x.Sq = q->size(1);
-    x.Sk = k->size(1);
-    x.Hq = q->size(2);
-    x.Hk = k->size(2);
-    x.D = D;
-    x.n_pos = c ? c->size(0) : 0;
-    x.q_offset = PyLong_AsLongLong(a[7]);
-    x.k_offset = PyLong_AsLongLong(a[8]);
+    const int64_t offset = PyLong_AsLongLong(a[7]), k_offset = PyLong_AsLongLong(a[8]);
     if (PyErr_Occurred()) return nullptr;
-    if (pos) {
-      x.pos_strides[0] = pos->stride(0);
-      x.pos_strides[1] = pos->stride(1);
+    const double eps = PyFloat_AS_DOUBLE(a[9]);
+    const at::Tensor no;
+    auto or_none = [&](const Arg& x) -> const at::Tensor& { return x ? *x.t : no; };
+    at::Tensor qo, ko;
+    if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(qw) || wants_grad(kw))) {
+      try {
+        auto maybe = [](const Arg& x) { return x ? std::optional<at::Tensor>(*x.t) : std::nullopt; };
+        auto out = NormRopeFn::apply(*q.t, *k.t, maybe(qw), maybe(kw), maybe(c), maybe(s), maybe(pos), offset,
+                                     k_offset, eps);
+        qo = std::move(out[0]);
+        ko = std::move(out[1]);
+      } catch (const Status& e) {
+        return PyLong_FromLong(e.rc);
+      }
+    } else {
+      qo = at::empty_like(*q.t);
+      ko = at::empty_like(*k.t);
+      auto x = norm_rope_args(*q.t, *k.t, or_none(qw), or_none(kw), or_none(c), or_none(s), or_none(pos), offset,
+                              k_offset, eps);
+      set_outputs(x, qo, ko);
+      if (const int rc = g_norm_rope(&x)) return PyLong_FromLong(rc);
     }
-    seq_strides(x.q_strides, *q.t);
-    seq_strides(x.k_strides, *k.t);
-    seq_strides(x.q_out_strides, qo);
-    seq_strides(x.k_out_strides, ko);
-    x.eps = PyFloat_AS_DOUBLE(a[9]);
-    x.stream = stream_of(dev);
-    if (const int rc = g_norm_rope(&x)) return PyLong_FromLong(rc);
     PyObject* out = PyTuple_New(2);
     if (!out) return nullptr;
     PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(qo)));
@@ -326,21 +450,24 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// bind(norm_rope, append, attend, attend workspace): the library's functions, as addresses
+// bind(norm_rope, its backward and that one's workspace size, append, attend and its workspace
+//      size): the library's functions, as addresses
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 4) {
-    PyErr_SetString(PyExc_TypeError, "bind takes four addresses");
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError, "bind takes six addresses");
     return nullptr;
   }
-  void* p[4];
-  for (int i = 0; i < 4; ++i) {
+  void* p[6];
+  for (int i = 0; i < 6; ++i) {
     p[i] = PyLong_AsVoidPtr(a[i]);
     if (PyErr_Occurred()) return nullptr;
   }
   g_norm_rope = reinterpret_cast<int (*)(const mlxp_qk_norm_rope_args*)>(p[0]);
-  g_append = reinterpret_cast<int (*)(const mlxp_paged_append_args*)>(p[1]);
-  g_attn = reinterpret_cast<int (*)(const mlxp_quant_paged_attn_args*)>(p[2]);
-  g_attn_ws = reinterpret_cast<size_t (*)(const mlxp_quant_paged_attn_args*)>(p[3]);
+  g_norm_rope_bwd = reinterpret_cast<int (*)(const mlxp_qk_norm_rope_args*)>(p[1]);
+  g_norm_rope_ws = reinterpret_cast<size_t (*)(int64_t)>(p[2]);
+  g_append = reinterpret_cast<int (*)(const mlxp_paged_append_args*)>(p[3]);
+  g_attn = reinterpret_cast<int (*)(const mlxp_quant_paged_attn_args*)>(p[4]);
+  g_attn_ws = reinterpret_cast<size_t (*)(const mlxp_quant_paged_attn_args*)>(p[5]);
   Py_RETURN_NONE;
 }
 

@@ -158,7 +158,8 @@ def calls():
             raise ImportError("mlx_primitives/_host.so is missing or does not match this torch; build it "
                               "with `python mlx-primitives_b200/csrc/build.py`") from e
         _host.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
-            L.mlxp_qk_norm_rope, L.mlxp_paged_append, L.mlxp_quant_paged_attn,
+            L.mlxp_qk_norm_rope, L.mlxp_qk_norm_rope_bwd, L.mlxp_qk_norm_rope_bwd_workspace_size,
+            L.mlxp_paged_append, L.mlxp_quant_paged_attn,
             L.mlxp_quant_paged_attn_workspace_size)))
         _calls = _host
     return _calls
