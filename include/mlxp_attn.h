@@ -419,6 +419,7 @@ size_t mlxp_qk_norm_rope_bwd_workspace_size(int64_t D);
  * NaN stays NaN in e4m3 and is 0 in int8.
  *
  * A block that receives tokens must be listed once: sequences may share only blocks that are full.
+ * k_pool and v_pool (and the scales) are different memory.
  */
 typedef struct mlxp_paged_append_args {
   uint64_t size;
@@ -450,7 +451,8 @@ int mlxp_paged_append(const mlxp_paged_append_args* args);
  * the query (before it; both sides when not causal).  ALiBi adds slope[h] * (t - position).
  * A query without keys, and rows past query_lens, are zeros.  q and o: fp32, bf16 or fp16, rows
  * 16-byte aligned; pools 16-byte aligned with strides that are multiples of 16; D 32, 64 or 128.
- * Scales are taken as of magnitude 2^-100 to 2^100.
+ * Scales are taken as finite, of magnitude 2^-100 to 2^100.  A NaN or infinite value that some row
+ * of a sequence sees may reach the others of that call.
  */
 typedef struct mlxp_quant_paged_attn_args {
   uint64_t size;

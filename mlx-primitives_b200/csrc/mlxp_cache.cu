@@ -301,6 +301,8 @@ int mlxp_paged_append(const mlxp_paged_append_args* a) {
                 (long long)a->bt_stride, (long long)a->max_blocks);
   if (quant && a->num_blocks > 0 && (!a->k_scales || !a->v_scales))
     return fail(MLXP_ERR_INVALID, "8-bit pools need their scales");
+  if (a->num_blocks > 0 && (a->k_pool == a->v_pool || (quant && a->k_scales == a->v_scales)))
+    return fail(MLXP_ERR_INVALID, "keys and values must go to different pools and scales");
 
   AppendParams p{};
   p.q = a->q;

@@ -51,13 +51,14 @@ def quantized_paged_attention(
 
     k_pool, v_pool: (num_blocks, block_size, kv_heads, head_dim) float8_e4m3fn or int8, heads a
     multiple of kv_heads, 16-byte aligned with strides that are multiples of 16; k_scales,
-    v_scales: (num_blocks, kv_heads) float32, of magnitude 2^-100 to 2^100.  block_tables:
+    v_scales: (num_blocks, kv_heads) float32, finite, of magnitude 2^-100 to 2^100.  block_tables:
     (batch, max_blocks), ids outside [0, num_blocks) are missing blocks.  context_lens: (batch,)
     cached tokens, the queries' own among them.  ``query_lens`` (batch,): queries of each sequence
     (default seq_q); rows behind them come back as zeros, as do rows that see no key.
     ``window_size`` W keeps keys at most W positions away, as ``sliding_window_attention`` does.
-    ALiBi adds slope[h] * (key position - query position).  Returns q's shape and dtype.  Not
-    differentiable.
+    ALiBi adds slope[h] * (key position - query position).  Returns q's shape and dtype.  Rows and
+    blocks behind the contexts may hold anything; a NaN or infinity among a sequence's own values
+    may reach all its rows, also those that do not see it.  Not differentiable.
     """
     if alibi_slopes is None and (window_size is None or window_size >= 0):
         out = _lib.calls().attend(q, k_pool, v_pool, k_scales, v_scales, block_tables, context_lens,

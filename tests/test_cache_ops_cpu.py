@@ -93,14 +93,15 @@ def test_c_abi_refuses_before_any_launch():
         assert norm(**kw) in (_lib.MLXP_ERR_INVALID, _lib.MLXP_ERR_UNSUPPORTED)
         assert why in L.mlxp_last_error(), (kw, L.mlxp_last_error())
 
-    def append(cache=1, B=1, block=16, mb=4, n_pos=64, scales=16, bts=4, k=16):
+    def append(cache=1, B=1, block=16, mb=4, n_pos=64, scales=16, bts=4, k=16, v_pool=32, v_scales=32):
         return L.mlxp_paged_append(APPEND.pack(
-            k, 16, 0, 0, 16, 16, scales, scales, 16, 16, 0, 0, 0, 16, 16, 1, cache, 0, 0, B, 1, 0,
+            k, 16, 0, 0, 16, v_pool, scales, v_scales, 16, 16, 0, 0, 0, 16, 16, 1, cache, 0, 0, B, 1, 0,
             1, 64, 8, block, mb, bts, n_pos, *[64] * 12, *[64] * 3, 1, 1, 1e-6, 0))
 
     for kw, why in [(dict(cache=2), b"dtype"), (dict(cache=3, scales=0), b"scales"),
                     (dict(n_pos=63), b"tables"), (dict(block=0), b"invalid shape"),
                     (dict(B=2, bts=3), b"stride"), (dict(k=0), b"non-null"),
+                    (dict(v_pool=16), b"different"), (dict(cache=3, v_scales=16), b"different"),
                     (dict(mb=1 << 30, n_pos=1 << 40), b"too large")]:
         assert append(**kw) == _lib.MLXP_ERR_INVALID
         assert why in L.mlxp_last_error(), (kw, L.mlxp_last_error())
