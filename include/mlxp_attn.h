@@ -404,7 +404,7 @@ size_t mlxp_qk_norm_rope_bwd_workspace_size(int64_t D);
 
 /*
  * New keys and values into a paged pool (the pools mlxp_paged_attn and mlxp_quant_paged_attn
- * read), keys, and queries beside them, normed and rotated on the way: one launch.  Token i of
+ * read), keys, and queries beside them, normed and rotated on the way.  Token i of
  * sequence b (i < new_lens[b]) has position pos = context_lens[b] + i and goes to row
  * pos % block_size of pool block block_tables[b][pos / block_size]; where the position is
  * negative or past the table, or the block id outside [0, num_blocks), the token is dropped.
@@ -415,8 +415,8 @@ size_t mlxp_qk_norm_rope_bwd_workspace_size(int64_t D);
  * (block, head) multiplies the codes.  A block whose first row is among the new tokens takes the
  * least power of two s >= 2^-126 with amax <= qmax * s over its new tokens (finite values; qmax
  * 448 or 127); a block that holds tokens already keeps its scale, or takes s where that is larger
- * and its earlier codes are rescaled.  Codes are round-to-nearest-even of value / scale, clamped to +-qmax;
- * NaN stays NaN in e4m3 and is 0 in int8.
+ * and its earlier codes are rescaled.  Codes are round-to-nearest-even of value / scale, clamped
+ * to +-qmax; NaN stays NaN in e4m3 and is 0 in int8.
  *
  * A block that receives tokens must be listed once: sequences may share only blocks that are full.
  * k_pool and v_pool (and the scales) are different memory.

@@ -1,5 +1,5 @@
 // cache_append.cuh — new keys and values into a paged K/V pool, the keys (and the queries beside
-// them) normed and rotated on the way, in one launch.
+// them) normed and rotated on the way, in one launch (long prompts into 8-bit pools: two).
 //
 // Token i of sequence b (i < new_lens[b]) has position pos = context_lens[b] + i and goes to row
 // pos % block_size of pool block block_tables[b][pos / block_size].  A position below 0 or past
@@ -22,8 +22,13 @@
 // One unit is (sequence, touched block, head, K or V), taken by WPU warps: they read the block's
 // new rows once and keep them (16 bf16 rows of 128 a warp: blocks of 16 need no other warp), in
 // registers as loaded and in shared memory as computed, until amax is known, on which they agree
-// through shared memory where they are several.  A block of more rows than eight warps hold is read a second time
-// (from L2).  Bound by HBM for prompts, by latency for single tokens.
+// through shared memory where they are several.  A block of more rows than eight warps hold is
+// read a second time (from L2).
+//
+// What bounds it: latency for single tokens (8 of them 3 us into 16-bit pools, 4.4 into e4m3: table
+// entry, scale, rows, maximum, old codes, one after the other); for prompts HBM on the query side
+// (32 heads of 128, 17.6 K ragged tokens: 75 us, 5.4 TB/s) and issue on the block side (2 x 8
+// heads of the same tokens: 56 us, 27.8 M warp instructions; 17 by its bytes).
 #pragma once
 
 #include <cuda_fp8.h>

@@ -91,6 +91,13 @@ void seq_strides(int64_t (&to)[3], const at::Tensor& t) {
   to[2] = t.stride(1);
 }
 
+// Like x, which has unit dim stride, as the result has: where x overlaps itself (an unfolded
+// view), empty_like may order the dimensions otherwise.
+at::Tensor rows_like(const at::Tensor& x) {
+  at::Tensor t = at::empty_like(x);
+  return t.stride(3) == 1 ? t : at::empty(x.sizes(), x.options());
+}
+
 void* stream_of(int64_t dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
 
 PyObject* none() { Py_RETURN_NONE; }
@@ -187,7 +194,7 @@ struct NormRopeFn : torch::autograd::Function<NormRopeFn> {
     const at::Tensor no;
     const at::Tensor &qw = qw_ ? *qw_ : no, &kw = kw_ ? *kw_ : no, &c = c_ ? *c_ : no, &s = s_ ? *s_ : no,
                      &pos = pos_ ? *pos_ : no;
-    at::Tensor qo = at::empty_like(q), ko = at::empty_like(k);
+    at::Tensor qo = rows_like(q), ko = rows_like(k);
     auto x = norm_rope_args(q, k, qw, kw, c, s, pos, offset, k_offset, eps);
     set_outputs(x, qo, ko);
     if (const int rc = g_norm_rope(&x)) throw Status{rc};
@@ -209,8 +216,8 @@ struct NormRopeFn : torch::autograd::Function<NormRopeFn> {
     variable_list out(10);
     {
       at::NoGradGuard no_grad;
-      if (g[0].defined()) out[0] = at::empty_like(q);
-      if (g[1].defined()) out[1] = at::empty_like(k);
+      if (g[0].defined()) out[0] = rows_like(q);
+      if (g[1].defined()) out[1] = rows_like(k);
       if (ctx->saved_data["dqw"].toBool()) out[2] = at::empty_like(qw);
       if (ctx->saved_data["dkw"].toBool()) out[3] = at::empty_like(kw);
       auto x = norm_rope_args(q, k, qw, kw, saved[4], saved[5], saved[6], ctx->saved_data["offset"].toInt(),
@@ -286,8 +293,8 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return PyLong_FromLong(e.rc);
       }
     } else {
-      qo = at::empty_like(*q.t);
-      ko = at::empty_like(*k.t);
+      qo = rows_like(*q.t);
+      ko = rows_like(*k.t);
       auto x = norm_rope_args(*q.t, *k.t, or_none(qw), or_none(kw), or_none(c), or_none(s), or_none(pos), offset,
                               k_offset, eps);
       set_outputs(x, qo, ko);
@@ -341,7 +348,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     x.size = sizeof(x);
     at::Tensor qo;
     if (q) {
-      qo = at::empty_like(*q.t);
+      qo = rows_like(*q.t);
       x.q = q.data();
       x.q_out = qo.data_ptr();
       x.Hq = q->size(2);

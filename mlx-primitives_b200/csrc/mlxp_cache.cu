@@ -77,7 +77,8 @@ constexpr int bwd_steps() { return R::kWide ? 2 : 1; }
 
 // From this many query units an SM, appends to 8-bit pools take two launches: the query rows run
 // at three CTAs an SM in a kernel of their own, at two beside the block units, whose registers
-// they share (8 ragged prompts, 17.6 K tokens of 32 + 2 x 8 heads of 128: 173 us in one launch).
+// they share (8 ragged prompts, 17.6 K tokens of 32 + 2 x 8 heads of 128: 131 us in two launches,
+// 173 in one; below it the second launch costs more than it gives).
 constexpr long long kSplitUnits = 64;
 
 int launched(const char* what) {

@@ -18,10 +18,14 @@ MLXP_INTERNAL int qa_rows_launch(int64_t dtype, int64_t D, bool int8, const QaPa
 
 namespace {
 
-#ifndef QR_FROM
-#define QR_FROM 64
-#endif
-constexpr int kRowsFrom = QR_FROM;
+// Query rows a pool head from which the many-row kernel (tcgen05, 256 rows a unit) is taken.  It
+// reads and converts the codes once for all of a unit's rows, the other once for every 16.
+// Measured at 8 heads of 128, e4m3, four contexts of 8 K / 64 of 2 K / one of 1000 tokens:
+//   48 rows   62 us against  82 / 283 against 219 / 19 against 21
+//   64        63 against  92     / 283 against 275 / 19 against 21
+//  128        70 against 147     / 295 against 502 / 21 against 26
+//  256        91 against 254     / 320 against 949 / 27 against 37
+constexpr int kRowsFrom = 64;
 
 struct QaPlan {
   bool many;         // the many-row kernel
@@ -35,8 +39,8 @@ struct QaPlan {
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // CTAs an SM holds (the launch bounds below are the same numbers).  Three rather than the four
-// that 128 registers a thread allow: four contexts of 128K tokens 185 us against 191, 48 ragged
-// ones at head_dim 64 37 against 40, at two 239 and 43.
+// that 128 registers a thread allow: four contexts of 128 K tokens 180 us against 190, 48 ragged
+// ones at head_dim 64 35 against 40, at two 239 and 43.
 template <int D, int NT, bool SPLIT>
 constexpr int qa_min_ctas() {
   return SPLIT && D == 128 ? 2 : 3;
@@ -94,14 +98,14 @@ QaPlan qa_plan(const mlxp_quant_paged_attn_args* a, int sms, QaParams& p) {
     p.HG = p.Hk;
     n.per_sm = 1;
   } else {
-  // 16 rows a warp where there are more than 8 (the codes are then converted once for both
-  // halves); the split operands of fp32 leave registers for 8
-  n.nt = p.R > 8 && a->dtype != MLXP_DTYPE_FP32 ? 2 : 1;
-  n.per_sm = qa_ctas(a->dtype, a->D, n.nt);
-  p.rows = std::min(p.R, 8 * n.nt);
-  p.RT = (p.R + 8 * n.nt - 1) / (8 * n.nt);
-  p.HP = p.Hk % 4 == 0 ? 4 : p.Hk % 2 == 0 ? 2 : 1;
-  p.HG = p.Hk / p.HP;
+    // 16 rows a warp where there are more than 8 (the codes are then converted once for both
+    // halves); the split operands of fp32 leave registers for 8
+    n.nt = p.R > 8 && a->dtype != MLXP_DTYPE_FP32 ? 2 : 1;
+    n.per_sm = qa_ctas(a->dtype, a->D, n.nt);
+    p.rows = std::min(p.R, 8 * n.nt);
+    p.RT = (p.R + 8 * n.nt - 1) / (8 * n.nt);
+    p.HP = p.Hk % 4 == 0 ? 4 : p.Hk % 2 == 0 ? 2 : 1;
+    p.HG = p.Hk / p.HP;
   }
   const int chunk = n.many ? kQrKeys : kQaChunk;
   const long long chunks = std::max<long long>(1, (cap + chunk - 1) / chunk + 1);
@@ -286,7 +290,7 @@ int mlxp_quant_paged_attn(const mlxp_quant_paged_attn_args* a) {
   p.p_scale = n.many ? 1.f : kQaPScale;
   p.causal = a->causal ? 1 : 0;
   p.bs_pow2 = (p.block_size & (p.block_size - 1)) == 0;
-  p.window = a->window;
+  p.window = std::min<long long>(a->window, 1LL << 40);  // positions are below 2^32: room to add
   p.scale_log2 = (float)(a->scale * 1.4426950408889634);
   const bool int8 = a->cache_dtype == MLXP_DTYPE_INT8;
   const cudaStream_t s = (cudaStream_t)a->stream;

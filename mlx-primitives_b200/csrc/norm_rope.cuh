@@ -16,7 +16,9 @@
 // a token's heads (or U steps of them where there are few tokens): they share a position, so its
 // table rows, which would cost twice the bytes of the data itself in L1, and the weights are
 // loaded once.  Arithmetic is on pairs (fma.rn.f32x2).  Both kernels are bound by HBM: the
-// forward reads and writes each element once, the backward reads x and g_out and writes dx.
+// forward reads and writes each element once, the backward reads x and g_out and writes dx.  2 x
+// 16384 tokens of 32 + 32 heads of 128 in bf16: 183 us (5.9 TB/s, 90 % of a copy's rate) and 278
+// (5.8 TB/s); units of rows rather than of tokens and scalar arithmetic took 811 together.
 #pragma once
 
 #include <type_traits>

@@ -17,9 +17,10 @@
 //
 // How the codes get there.  Where the block size is a multiple of 16 a tile is one TMA box of K
 // and one of V (16 rows of one head), three or four stages in flight a warp, each on its own
-// mbarrier: 87 % of the measured HBM rate at four contexts of 128K tokens.  Loads into registers
-// (257 us there against 190) left a warp one tile ahead, and cp.async (284 us) kept the load
-// path busy with 28 instructions a tile.  Other block sizes do take cp.async, every lane copying
+// mbarrier.  Four contexts of 128 K tokens, 8 heads of 128 (1.07 GB of codes): 180 us, 170 of them
+// in this kernel, 92 % of the measured HBM rate; four CTAs an SM instead of three 190 us, loads
+// into registers 257 (a warp is then one tile ahead), cp.async 284 (28 instructions a tile keep
+// the load path busy).  Eight of 4 K, 32 heads (269 MB): 52 us and 5 for the merge.  Other block sizes do take cp.async, every lane copying
 // the bytes that it reads itself.  The order of a dot product's terms is free, so the fragments
 // are filled straight from the rows: of a K row the four lanes c of a row group hold 16-byte
 // pieces, each word of which is one k16 step's two pairs; of a V row the eight lanes g hold
@@ -886,10 +887,13 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
 }
 
 // Merges the partials of the units that more than one CTA worked on.  Block x looks at main CTA
-// x + 1: where that is the second CTA of a unit, it merges the unit's rows.  Up to 32 partials a
-// warp takes a row to itself; the rows of a unit split further (few units, long contexts) are
-// taken by all the block's warps together.
+// x + 1: where that is the second CTA of a unit, it merges the unit's rows.  A warp takes a row to
+// itself, or the block's warps share one: from 5 partials where all blocks run at once (a single
+// short context: 3.9 us, 5.5 with a warp a row), from 33 otherwise (48 contexts to 9000 with 9
+// partials each: 6.6 us, 9.1 with a block a row).  Blocks that look at eight CTAs each instead
+// took 1 to 2 us longer, but for the longest contexts (8.3 us for 9.8).
 constexpr int kQaMergeWarps = 8;
+constexpr unsigned kQaMergeResident = 1024;  // blocks of 256 threads that run at once
 
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kQaMergeWarps) quant_attn_merge_kernel(const QaParams p) {
@@ -904,7 +908,7 @@ __global__ void __launch_bounds__(32 * kQaMergeWarps) quant_attn_merge_kernel(co
   const int sub = lane / LPR, d = (lane % LPR) * 4;
   const int b = info.v / p.RT, r0 = (info.v - b * p.RT) * p.rows;
   const int qlen = p.query_lens ? p.query_lens[b] : p.Sq;
-  const bool together = info.parts > 32;
+  const bool together = info.parts > (gridDim.x * gridDim.y <= kQaMergeResident ? 4 : 32);
   const int team = together ? kQaMergeWarps : 1, me = together ? warp : 0;  // warps a row, this one's place
   const int stride = together ? gridDim.y : gridDim.y * kQaMergeWarps;
   for (int y = together ? blockIdx.y : blockIdx.y * kQaMergeWarps + warp; y < p.HP * p.rows; y += stride) {

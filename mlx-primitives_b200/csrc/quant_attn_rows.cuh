@@ -3,8 +3,12 @@
 //
 // The same function, precision and split of work as quant_attn.cuh (which see), for more query
 // rows a pool head than its 16-row tiles are good for: a unit is 256 rows (two TMEM tiles of 128)
-// of one pool head, a chunk 128 keys.  What bounds it is the tensor pipe, then the exponentials:
-// 4 * 128 * 128 * D flops a tile and key chunk against 128 * 128 exponentials.
+// of one pool head, a chunk 128 keys.  By work it is bound by the tensor pipe (4 * 128 * 128 * D
+// flops a tile and key chunk, 1450 cycles at D = 128), then by the exponentials (128 * 128 of
+// them, 1024 cycles); as it stands by the chain that a tile's chunk runs through: scores out of
+// TMEM, maximum, exponentials, weights back, PV, the next QK, 5.5 to 6 K cycles, of which the two
+// tiles hide half.  Four sequences of 512 queries and contexts to 8 K, 32 heads over 8 of 128:
+// 325 us and 20 for the merge, 530 TFLOP/s.
 //
 // The codes become fp16 (exactly) on their way into shared memory, once for both tiles: the MMA
 // reads 16-bit operands, and 8-bit queries would lose what the cache kept.  Scales stay out of
@@ -42,11 +46,6 @@ static_assert(128 * (2 * kQrRegsSoftmax + kQrRegsConvert) <= 384 * 168, "registe
 constexpr int kQrRows = 256, kQrKeys = 128;
 constexpr float kQrPLog = 8.f;  // log2 of the weights' factor; the sums l carry it too
 constexpr float kQrHeadroom = 7.f;
-#ifndef QR_POLY
-#define QR_POLY 0
-#endif
-// of every 8 pairs of weights, exponentiated on the FMA pipe (exp2_poly2, 7.2e-5 off at most)
-constexpr int kQrPolyPerOct = QR_POLY;
 constexpr int kSiteQuantRows = 13;
 
 template <int D>
@@ -255,152 +254,144 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
       named_bar_sync(1 + t, 128);  // the tile's Q is in place
       float m = -1e30f, l = 0.f;
       bool ok = true;
-      {
-        if (issuer) ok = issue_qk(cnt, alone);
-        for (int j = u.ch0; j < u.ch1; ++j) {
-          const int c = cnt + j - u.ch0;
-          if (ok) ok = mbar_wait(BAR(C::B_SF + t), n_s & 1, wctx, kSiteQuantRows);
-          ok = __all_sync(0xffffffffu, ok);
-          ++n_s;
-          tc_fence_after();
-          if (ok) {
-            const int key0 = (u.r.c0 + j) * kQrKeys;
-            const float4* sc = s_scale + (c & 3) * 8;
-            uint32_t x[4][32];
-            tmem_ld_x32(tS, x[0]);
-            tmem_ld_x32(tS + 32, x[1]);
-            tmem_ld_x32(tS + 64, x[2]);
-            tmem_ld_x32(tS + 96, x[3]);
-            uint32_t groups = s_mask[c & 3];  // bits 0, 1 of each byte
-            groups = (groups & 3u) | (groups >> 6 & 12u) | (groups >> 12 & 48u) | (groups >> 18 & 192u);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 4; ++k) reg_fence(x[k]);
-            if (key0 < u.r.flo || key0 + kQrKeys > u.r.fhi || groups != 0xffu) {
-              const int from = lo - key0;
-              const unsigned width = (unsigned)max(hi - lo, 0);
-#pragma unroll
-              for (int e = 0; e < 128; ++e)
-                if ((unsigned)(e - from) >= width || !(groups >> (e >> 4) & 1u)) x[e >> 5][e & 31] = 0xff800000u;
-            }
-            float mloc = -INFINITY;
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {
-              const uint32_t* v = x[g >> 1] + 16 * (g & 1);
-              float mx = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
-#pragma unroll
-              for (int e = 2; e < 16; e += 2) mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-              mloc = fmaxf(mloc, fmaf(mx, fmaxf(sc[g].x * qs, 1.2e-38f), sc[g].y));
-            }
-            const bool resc = mloc > m + kQrHeadroom;
-            float alpha = 1.f;
-            if (resc) {
-              alpha = ex2_approx(m - mloc);
-              m = mloc;
-            }
-            // weight = 2^(s f - m + log2 |vs| + 8): what multiplies V's codes; the sum l of the
-            // weights without vs is taken a group at a time.  The weights go over the scores'
-            // first 64 columns as fp16.
-            float sum = 0.f;
-            const float base = kQrPLog - m;
-            // The two tiles' warps of a scheduler take turns here.  Left alone they fall into
-            // step, both exponentiating (half as fast each), then both waiting for the MMAs.
-            if (!alone) {
-              if (t == 1 || n_t > 0) ok = mbar_wait(turn_mine, (n_t - 1 + t) & 1, wctx, kSiteQuantRows);
-              ++n_t;
-              __syncwarp();
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int g = 0; g < 2; ++g) {
-                const float4 sg = sc[2 * k + g];
-                const float f = fmaxf(sg.x * qs, 1.2e-38f), add = sg.y + base;  // f > 0: -inf stays -inf
-                float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const uint32_t* v = x[k] + 16 * g + 2 * e;
-                  const float2 z = fma2(make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])), make_float2(f, f),
-                                        make_float2(add, add));
-                  float2 y;
-                  if (e < kQrPolyPerOct) {
-                    y = exp2_poly2(z);
-                  } else {
-                    y.x = ex2_approx(z.x);
-                    y.y = ex2_approx(z.y);
-                  }
-                  acc[e & 1] = add2(acc[e & 1], y);
-                  pk[8 * g + e] = qa_pack(y.x, y.y);
-                }
-                const float2 s2 = add2(acc[0], acc[1]);
-                sum = fmaf(s2.x + s2.y, sg.z, sum);
-              }
-              tmem_st_x16(tS + 16 * k, pk);
-            }
-            if (!alone) {
-              __syncwarp();
-              if (lane == 0) mbar_arrive(turn_other);
-            }
-            if (j > u.ch0 && __any_sync(0xffffffffu, resc)) {
-#pragma unroll 1
-              for (int e = 0; e < D / 32; ++e) {
-                tmem_ld_x32(tO + e * 32, x[0]);
-                tmem_wait_ld();
-                reg_fence(x[0]);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) x[0][i] = __float_as_uint(__uint_as_float(x[0][i]) * alpha);
-                tmem_st_x32(tO + e * 32, x[0]);
-              }
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            l = fmaf(l, alpha, sum);
-          }
-          // the tile's weights are in place; its warps go on together or not at all
-          ok = named_bar_and(1 + t, 128, ok);
-          if (!ok) break;
-          if (issuer) {
-            const bool more = j + 1 < u.ch1;
-            ok = issue_pv(c, j == u.ch0, alone);
-            if (!more) tc_commit(BAR(C::B_OF + t));
-            else if (ok) ok = issue_qk(c + 1, alone);
-          }
-        }
-        if (ok) ok = mbar_wait(BAR(C::B_OF + t), n_o & 1, wctx, kSiteQuantRows);
-        ++n_o;
+      if (issuer) ok = issue_qk(cnt, alone);
+      for (int j = u.ch0; j < u.ch1; ++j) {
+        const int c = cnt + j - u.ch0;
+        if (ok) ok = mbar_wait(BAR(C::B_SF + t), n_s & 1, wctx, kSiteQuantRows);
         ok = __all_sync(0xffffffffu, ok);
+        ++n_s;
         tc_fence_after();
         if (ok) {
-          const long long pr = u.slot * p.rows + t * 128 + row;
-          const float inv = 1.f / l;
-          const bool some = live && l != 0.f;
-          T* out = static_cast<T*>(p.o) + u.b * p.o_sb + (long long)h * p.o_sh + (long long)qi * p.o_ss;
-#pragma unroll 1
-          for (int e = 0; e < D / 32; ++e) {
-            uint32_t o[32];
-            tmem_ld_x32(tO + e * 32, o);
-            tmem_wait_ld();
-            reg_fence(o);
-            if (qrow < p.R) {
-              if (u.whole) {
+          const int key0 = (u.r.c0 + j) * kQrKeys;
+          const float4* sc = s_scale + (c & 3) * 8;
+          uint32_t x[4][32];
+          tmem_ld_x32(tS, x[0]);
+          tmem_ld_x32(tS + 32, x[1]);
+          tmem_ld_x32(tS + 64, x[2]);
+          tmem_ld_x32(tS + 96, x[3]);
+          uint32_t groups = s_mask[c & 3];  // bits 0, 1 of each byte
+          groups = (groups & 3u) | (groups >> 6 & 12u) | (groups >> 12 & 48u) | (groups >> 18 & 192u);
+          tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                  alignas(16) T v[8];
+          for (int k = 0; k < 4; ++k) reg_fence(x[k]);
+          if (key0 < u.r.flo || key0 + kQrKeys > u.r.fhi || groups != 0xffu) {
+            const int from = lo - key0;
+            const unsigned width = (unsigned)max(hi - lo, 0);
 #pragma unroll
-                  for (int z = 0; z < 8; ++z) v[z] = from_f<T>(some ? __uint_as_float(o[i + z]) * inv : 0.f);
-                  *reinterpret_cast<uint4*>(out + 32 * e + i) = *reinterpret_cast<const uint4*>(v);
-                }
-              } else {
+            for (int e = 0; e < 128; ++e)
+              if ((unsigned)(e - from) >= width || !(groups >> (e >> 4) & 1u)) x[e >> 5][e & 31] = 0xff800000u;
+          }
+          float mloc = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 32; i += 4)
-                  *reinterpret_cast<uint4*>(p.o_part + pr * D + 32 * e + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int g = 0; g < 8; ++g) {
+            const uint32_t* v = x[g >> 1] + 16 * (g & 1);
+            float mx = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
+#pragma unroll
+            for (int e = 2; e < 16; e += 2) mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+            mloc = fmaxf(mloc, fmaf(mx, fmaxf(sc[g].x * qs, 1.2e-38f), sc[g].y));
+          }
+          const bool resc = mloc > m + kQrHeadroom;
+          float alpha = 1.f;
+          if (resc) {
+            alpha = ex2_approx(m - mloc);
+            m = mloc;
+          }
+          // weight = 2^(s f - m + log2 |vs| + 8): what multiplies V's codes; the sum l of the
+          // weights without vs is taken a group at a time.  The weights go over the scores'
+          // first 64 columns as fp16.
+          float sum = 0.f;
+          const float base = kQrPLog - m;
+          // The two tiles' warps of a scheduler take turns here.  Left alone they fall into
+          // step, both exponentiating (half as fast each), then both waiting for the MMAs.
+          if (!alone) {
+            if (t == 1 || n_t > 0) ok = mbar_wait(turn_mine, (n_t - 1 + t) & 1, wctx, kSiteQuantRows);
+            ++n_t;
+            __syncwarp();
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const float4 sg = sc[2 * k + g];
+              const float f = fmaxf(sg.x * qs, 1.2e-38f), add = sg.y + base;  // f > 0: -inf stays -inf
+              float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t* v = x[k] + 16 * g + 2 * e;
+                const float2 z = fma2(make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])), make_float2(f, f),
+                                      make_float2(add, add));
+                const float2 y = make_float2(ex2_approx(z.x), ex2_approx(z.y));
+                acc[e & 1] = add2(acc[e & 1], y);
+                pk[8 * g + e] = qa_pack(y.x, y.y);
               }
+              const float2 s2 = add2(acc[0], acc[1]);
+              sum = fmaf(s2.x + s2.y, sg.z, sum);
+            }
+            tmem_st_x16(tS + 16 * k, pk);
+          }
+          if (!alone) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(turn_other);
+          }
+          if (j > u.ch0 && __any_sync(0xffffffffu, resc)) {
+#pragma unroll 1
+            for (int e = 0; e < D / 32; ++e) {
+              tmem_ld_x32(tO + e * 32, x[0]);
+              tmem_wait_ld();
+              reg_fence(x[0]);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[0][i] = __float_as_uint(__uint_as_float(x[0][i]) * alpha);
+              tmem_st_x32(tO + e * 32, x[0]);
             }
           }
-          if (!u.whole && qrow < p.R) *reinterpret_cast<float2*>(p.ml_part + 2 * pr) = make_float2(m, l);
+          tmem_wait_st();
           tc_fence_before();
+          l = fmaf(l, alpha, sum);
         }
+        // the tile's weights are in place; its warps go on together or not at all
+        ok = named_bar_and(1 + t, 128, ok);
+        if (!ok) break;
+        if (issuer) {
+          const bool more = j + 1 < u.ch1;
+          ok = issue_pv(c, j == u.ch0, alone);
+          if (!more) tc_commit(BAR(C::B_OF + t));
+          else if (ok) ok = issue_qk(c + 1, alone);
+        }
+      }
+      if (ok) ok = mbar_wait(BAR(C::B_OF + t), n_o & 1, wctx, kSiteQuantRows);
+      ++n_o;
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      if (ok) {
+        const long long pr = u.slot * p.rows + t * 128 + row;
+        const float inv = 1.f / l;
+        const bool some = live && l != 0.f;
+        T* out = static_cast<T*>(p.o) + u.b * p.o_sb + (long long)h * p.o_sh + (long long)qi * p.o_ss;
+#pragma unroll 1
+        for (int e = 0; e < D / 32; ++e) {
+          uint32_t o[32];
+          tmem_ld_x32(tO + e * 32, o);
+          tmem_wait_ld();
+          reg_fence(o);
+          if (qrow < p.R) {
+            if (u.whole) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) {
+                alignas(16) T v[8];
+#pragma unroll
+                for (int z = 0; z < 8; ++z) v[z] = from_f<T>(some ? __uint_as_float(o[i + z]) * inv : 0.f);
+                *reinterpret_cast<uint4*>(out + 32 * e + i) = *reinterpret_cast<const uint4*>(v);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<uint4*>(p.o_part + pr * D + 32 * e + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
+          }
+        }
+        if (!u.whole && qrow < p.R) *reinterpret_cast<float2*>(p.ml_part + 2 * pr) = make_float2(m, l);
+        tc_fence_before();
       }
       cnt += u.ch1 - u.ch0;
       advance(u);

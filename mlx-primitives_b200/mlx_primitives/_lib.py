@@ -165,6 +165,13 @@ def calls():
     return _calls
 
 
+def rows_like(x: torch.Tensor) -> torch.Tensor:
+    """Empty, like x, which has unit last stride, as the result has: where x overlaps itself (an
+    unfolded view), empty_like may order the dimensions otherwise."""
+    t = torch.empty_like(x)
+    return t if t.stride(-1) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def last_error() -> str:
     msg = lib().mlxp_last_error()
     return msg.decode() if msg else ""

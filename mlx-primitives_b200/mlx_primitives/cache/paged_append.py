@@ -2,7 +2,7 @@
 
 The write side of the pools that ``paged_attention`` and ``quantized_paged_attention`` read.  The
 reference keeps that in its cache managers (mlx_primitives/cache/paged_attention.py:44-105
-takes pools that something else has filled); here it is one launch (mlxp_paged_append): the new
+takes pools that something else has filled); here it is one call (mlxp_paged_append): the new
 keys, and the queries beside them, are normed (where weights are given) and rotated in fp32 and
 written once, in the pools' type or as 8-bit codes.
 """
@@ -161,7 +161,7 @@ def paged_append(
         if qs[3] != 1:
             q = q.contiguous()
             qs = q.stride()
-        q_out = torch.empty_like(q)
+        q_out = _lib.rows_like(q)
         q_ptr, qo_ptr, qo = q.data_ptr(), q_out.data_ptr(), q_out.stride()
     elif q_weight is not None:
         raise ValueError("q_weight needs q")

@@ -115,7 +115,7 @@ def _dense(t):
 
 
 def _forward(dev, q, k, q_weight, k_weight, cos, sin, positions, offset, k_offset, eps):
-    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    q_out, k_out = _lib.rows_like(q), _lib.rows_like(k)
     with _lib.on_device(dev):
         rc = _lib.lib().mlxp_qk_norm_rope(_pack(
             dev, q, k, q_out, k_out, None, None, q_weight, k_weight, None, None, cos, sin,
@@ -139,8 +139,8 @@ class _QKNormRopeFn(torch.autograd.Function):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         dev, offset, k_offset, eps = ctx.args
         gq, gk = _dense(gq), _dense(gk)
-        dq = None if gq is None else torch.empty_like(q)
-        dk = None if gk is None else torch.empty_like(k)
+        dq = None if gq is None else _lib.rows_like(q)
+        dk = None if gk is None else _lib.rows_like(k)
         dqw = torch.empty_like(q_weight) if ctx.needs_input_grad[3] else None
         dkw = torch.empty_like(k_weight) if ctx.needs_input_grad[4] else None
         L = _lib.lib()
