@@ -20,11 +20,12 @@
 // mbarrier.  Four contexts of 128 K tokens, 8 heads of 128 (1.07 GB of codes): 180 us, 170 of them
 // in this kernel, 92 % of the measured HBM rate; four CTAs an SM instead of three 190 us, loads
 // into registers 257 (a warp is then one tile ahead), cp.async 284 (28 instructions a tile keep
-// the load path busy).  Eight of 4 K, 32 heads (269 MB): 52 us and 5 for the merge.  Other block sizes do take cp.async, every lane copying
-// the bytes that it reads itself.  The order of a dot product's terms is free, so the fragments
-// are filled straight from the rows: of a K row the four lanes c of a row group hold 16-byte
-// pieces, each word of which is one k16 step's two pairs; of a V row the eight lanes g hold
-// D / 8 bytes each, and a byte permute of two keys' words gives the pairs along keys.
+// the load path busy).  Eight of 4 K, 32 heads (269 MB): 52 us and 5 for the merge.  Other block
+// sizes do take cp.async, every lane copying the bytes that it reads itself.  The order of a dot
+// product's terms is free, so the fragments are filled straight from the rows: of a K row the four
+// lanes c of a row group hold 16-byte pieces, each word of which is one k16 step's two pairs; of a
+// V row the eight lanes g hold D / 8 bytes each, and a byte permute of two keys' words gives the
+// pairs along keys.
 //
 // Precision.  16-bit queries are scaled by a power of two a row to [1, 2) at most and held in
 // fp16 (bf16 values lose nothing but below 2^-25 of the row's largest); fp32 queries and
