@@ -15,12 +15,15 @@
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <cmath>
-#include <optional>
+#include <memory>
+#include <mutex>
 #include <stdexcept>
 #include <string>
 
@@ -129,10 +132,6 @@ PyObject* guarded(F&& f) {
 
 // ---- norm + rotation, with its gradient -------------------------------------------------------
 
-struct Status {  // of a launch inside the autograd function
-  int rc;
-};
-
 // What the forward and the backward have in common; undefined tensors are not there.
 mlxp_qk_norm_rope_args norm_rope_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw,
                                       const at::Tensor& kw, const at::Tensor& c, const at::Tensor& s,
@@ -186,42 +185,34 @@ void set_outputs(mlxp_qk_norm_rope_args& x, const at::Tensor& qo, const at::Tens
 
 using torch::autograd::variable_list;
 
-struct NormRopeFn : torch::autograd::Function<NormRopeFn> {
-  using Maybe = std::optional<at::Tensor>;
-  static variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
-                               const Maybe& qw_, const Maybe& kw_, const Maybe& c_, const Maybe& s_, const Maybe& pos_,
-                               int64_t offset, int64_t k_offset, double eps) {
-    const at::Tensor no;
-    const at::Tensor &qw = qw_ ? *qw_ : no, &kw = kw_ ? *kw_ : no, &c = c_ ? *c_ : no, &s = s_ ? *s_ : no,
-                     &pos = pos_ ? *pos_ : no;
-    at::Tensor qo = rows_like(q), ko = rows_like(k);
-    auto x = norm_rope_args(q, k, qw, kw, c, s, pos, offset, k_offset, eps);
-    set_outputs(x, qo, ko);
-    if (const int rc = g_norm_rope(&x)) throw Status{rc};
-    ctx->set_materialize_grads(false);
-    ctx->save_for_backward({q, k, qw, kw, c, s, pos});
-    ctx->saved_data["offset"] = offset;
-    ctx->saved_data["k_offset"] = k_offset;
-    ctx->saved_data["eps"] = eps;
-    ctx->saved_data["dqw"] = qw.defined() && qw.requires_grad();
-    ctx->saved_data["dkw"] = kw.defined() && kw.requires_grad();
-    return {qo, ko};
+// The graph's node.  A Node of its own rather than torch::autograd::Function: that one's context
+// and wrapping of outputs cost as much as the launches.
+struct NormRopeBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable q_, k_, qw_, kw_, c_, s_, pos_;
+  int64_t offset = 0, k_offset = 0;
+  double eps = 0;
+
+  std::string name() const override { return "QKNormRopeBackward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto* v : {&q_, &k_, &qw_, &kw_, &c_, &s_, &pos_}) v->reset_data();
   }
 
-  static variable_list backward(torch::autograd::AutogradContext* ctx, variable_list g) {
-    const auto saved = ctx->get_saved_variables();
-    const at::Tensor &q = saved[0], &k = saved[1], &qw = saved[2], &kw = saved[3];
+  variable_list apply(variable_list&& g) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    const at::Tensor q = q_.unpack(), k = k_.unpack(), qw = qw_.unpack(), kw = kw_.unpack(), c = c_.unpack(),
+                     s = s_.unpack(), pos = pos_.unpack();
     for (at::Tensor& t : g)
       if (t.defined() && t.stride(3) != 1) t = t.contiguous();
-    variable_list out(10);
+    variable_list out(4);
     {
-      at::NoGradGuard no_grad;
+      at::AutoDispatchBelowADInplaceOrView below;  // plain allocations
       if (g[0].defined()) out[0] = rows_like(q);
       if (g[1].defined()) out[1] = rows_like(k);
-      if (ctx->saved_data["dqw"].toBool()) out[2] = at::empty_like(qw);
-      if (ctx->saved_data["dkw"].toBool()) out[3] = at::empty_like(kw);
-      auto x = norm_rope_args(q, k, qw, kw, saved[4], saved[5], saved[6], ctx->saved_data["offset"].toInt(),
-                              ctx->saved_data["k_offset"].toInt(), ctx->saved_data["eps"].toDouble());
+      if (qw.defined() && task_should_compute_output(2)) out[2] = at::empty_like(qw);
+      if (kw.defined() && task_should_compute_output(3)) out[3] = at::empty_like(kw);
+      auto x = norm_rope_args(q, k, qw, kw, c, s, pos, offset, k_offset, eps);
       set_outputs(x, out[0], out[1]);
       if (g[0].defined()) {
         x.gq = g[0].data_ptr();
@@ -281,24 +272,34 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const double eps = PyFloat_AS_DOUBLE(a[9]);
     const at::Tensor no;
     auto or_none = [&](const Arg& x) -> const at::Tensor& { return x ? *x.t : no; };
+    const bool graph =
+        at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(qw) || wants_grad(kw));
     at::Tensor qo, ko;
-    if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(qw) || wants_grad(kw))) {
-      try {
-        auto maybe = [](const Arg& x) { return x ? std::optional<at::Tensor>(*x.t) : std::nullopt; };
-        auto out = NormRopeFn::apply(*q.t, *k.t, maybe(qw), maybe(kw), maybe(c), maybe(s), maybe(pos), offset,
-                                     k_offset, eps);
-        qo = std::move(out[0]);
-        ko = std::move(out[1]);
-      } catch (const Status& e) {
-        return PyLong_FromLong(e.rc);
-      }
-    } else {
+    {
+      at::AutoDispatchBelowADInplaceOrView below;  // plain allocations
       qo = rows_like(*q.t);
       ko = rows_like(*k.t);
-      auto x = norm_rope_args(*q.t, *k.t, or_none(qw), or_none(kw), or_none(c), or_none(s), or_none(pos), offset,
-                              k_offset, eps);
-      set_outputs(x, qo, ko);
-      if (const int rc = g_norm_rope(&x)) return PyLong_FromLong(rc);
+    }
+    auto x = norm_rope_args(*q.t, *k.t, or_none(qw), or_none(kw), or_none(c), or_none(s), or_none(pos), offset,
+                            k_offset, eps);
+    set_outputs(x, qo, ko);
+    if (const int rc = g_norm_rope(&x)) return PyLong_FromLong(rc);
+    if (graph) {
+      auto node = std::shared_ptr<NormRopeBackward>(new NormRopeBackward(), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(*q.t, *k.t, or_none(qw), or_none(kw)));
+      using torch::autograd::SavedVariable;
+      node->q_ = SavedVariable(*q.t, false);
+      node->k_ = SavedVariable(*k.t, false);
+      node->qw_ = SavedVariable(or_none(qw), false);
+      node->kw_ = SavedVariable(or_none(kw), false);
+      node->c_ = SavedVariable(or_none(c), false);
+      node->s_ = SavedVariable(or_none(s), false);
+      node->pos_ = SavedVariable(or_none(pos), false);
+      node->offset = offset;
+      node->k_offset = k_offset;
+      node->eps = eps;
+      torch::autograd::set_history(qo, node);
+      torch::autograd::set_history(ko, node);
     }
     PyObject* out = PyTuple_New(2);
     if (!out) return nullptr;

@@ -614,6 +614,45 @@ def test_norm_rope_of_unfolded_views():
         assert (a - b).abs().max() <= tol
 
 
+def test_norm_rope_graphs_kept_freed_and_modified():
+    """A kept graph runs twice, a freed one is refused, as are values changed since; inputs that need
+    no gradient get none, and hooks and accumulation see the same gradients."""
+    from mlx_primitives.kernels import qk_norm_rope
+
+    rs = np.random.RandomState(38)
+    q, k, w = _rand(rs, (2, 7, 4, 64), torch.bfloat16), _rand(rs, (2, 7, 2, 64), torch.bfloat16), _rand(rs, (64,), torch.float32)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, w, w)]
+    out = qk_norm_rope(*leaves)
+    g = [torch.ones_like(o) for o in out]
+    first = torch.autograd.grad(out, leaves, g, retain_graph=True)
+    again = torch.autograd.grad(out, leaves, g)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, leaves, g)
+    only = qk_norm_rope(leaves[0], k, w, leaves[3])
+    assert all(o.requires_grad for o in only)
+    dq, dkw = torch.autograd.grad(only, (leaves[0], leaves[3]), g)
+    assert torch.equal(dq, first[0]) and torch.equal(dkw, first[3])
+    seen = []
+    leaves[0].register_hook(seen.append)
+    for _ in range(2):
+        o = qk_norm_rope(leaves[0] * 1.0, *leaves[1:])
+        torch.autograd.backward(o, g)
+    assert torch.equal(seen[0], first[0]) and torch.equal(leaves[0].grad, first[0] * 2)
+    assert torch.equal(leaves[2].grad, first[2] * 2)
+    x = q * 1.0
+    x.requires_grad_(True)
+    y = x * 1.0
+    o = qk_norm_rope(y, k, w, w)
+    y.mul_(2.0)
+    with pytest.raises(RuntimeError):
+        o[0].sum().backward()
+    o = qk_norm_rope(x, k, w, w)[0]
+    o.mul_(2.0)  # the results may be changed
+    o.sum().backward()
+    assert torch.equal(x.grad, 2.0 * torch.autograd.grad(qk_norm_rope(x, k, w, w)[0].sum(), x)[0])
+
+
 def test_attention_many_rows_long_split_and_stale():
     """Units split over CTAs, several row tiles a pool head; stale rows of NaN codes; scales of
     many sizes and signs."""
