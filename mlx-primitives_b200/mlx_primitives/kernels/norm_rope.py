@@ -174,7 +174,9 @@ def qk_norm_rope(
     position ``offset`` + s (``k_offset`` + s for k, default ``offset``), or at ``positions``
     (batch, seq) where given: a negative position marks padding, whose row becomes zeros and has
     no gradient; one past the tables gives a row of NaN (it is read on the device, where it
-    cannot be refused).  head_dim is even and at most 256.
+    cannot be refused).  head_dim is even and at most 256.  As for every operator, a training step
+    is captured into a CUDA graph while no eager autograd graph of the same leaves is alive: their
+    accumulation belongs to the stream of the graph that made it.
     """
     out = _lib.calls().norm_rope(q, k, q_weight, k_weight, cos_cache, sin_cache, positions, offset,
                                  offset if k_offset is None else k_offset, eps)
