@@ -417,7 +417,9 @@ __global__ void __launch_bounds__(256, MINB) norm_rope_bwd_kernel(const NormRope
             const float sum = row_sum<R::LPR>(ss.x + ss.y), dot = row_sum<R::LPR>(sg.x + sg.y);
             const float r1 = rsqrtf(fmaf(sum, t.norm.inv_d, t.norm.eps));
             const float2 r = both(r1), m = both(-dot * t.norm.inv_d * r1 * r1);
-            if (pos >= 0) {  // a padding row's x may hold anything: it must not reach dw
+            // a padding row's x may hold anything, and a lane without a row has r = inf where eps
+            // is 0: neither must reach dw
+            if (pos >= 0 && h < last) {
 #pragma unroll
               for (int e = 0; e < R::NP; ++e) {
                 const float2 u = mul2(x1[e], r), z = mul2(x2[e], r);

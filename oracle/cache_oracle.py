@@ -49,7 +49,8 @@ def norm_rope_grad(gy, x, weight, cos, sin, pos, eps=1e-6):
     if weight is None:
         return g, None, None
     w = np.asarray(weight, np.float64)
-    r = 1.0 / np.sqrt((x * x).mean(-1, keepdims=True) + eps)
+    r = np.zeros(x.shape[:-1] + (1,))  # of padding rows: they add nothing, eps = 0 or not
+    np.divide(1.0, np.sqrt((x * x).mean(-1, keepdims=True) + eps), out=r, where=live)
     xh = x * r
     terms = g * xh
     gw = g * w

@@ -1,0 +1,43 @@
+"""The cache operators where they can go wrong beside tests/test_gpu_cache_ops.py: the limits of
+their scales, masks and sizes, autograd's other modes, and the ways a call can take to the kernels.
+Tolerances are those of that file, which derives them."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import cache_oracle as C
+from test_gpu_cache_ops import TYPES, _check_norm, _close, _n, _norm_case, _rand, _tables
+
+pytestmark = pytest.mark.gpu
+
+
+def _check_gradients(leaves, out, pos, cos, sin, eps, seed):
+    """Gradients of q, k and both weights against the oracle's, tolerances as in
+    test_norm_rope_gradients."""
+    q, k, qw, kw = leaves
+    rs = np.random.RandomState(seed)
+    gq, gk = _rand(rs, q.shape, q.dtype), _rand(rs, k.shape, k.dtype)
+    got = torch.autograd.grad(out, leaves, (gq, gk))
+    for x, w, g, dx, dw in ((q, qw, gq, got[0], got[2]), (k, kw, gk, got[1], got[3])):
+        want, wsum, wabs = C.norm_rope_grad(_n(g), _n(x), _n(w), _n(cos), _n(sin), pos, eps)
+        size = np.abs(_n(g)).max(-1, keepdims=True) * 3 / np.sqrt(
+            np.where((pos >= 0)[:, :, None, None], (np.nan_to_num(_n(x)) ** 2).mean(-1, keepdims=True), 1) + eps)
+        _close(dx, want, x.dtype, 2.0 ** -19 * size)
+        chain = x.shape[0] * x.shape[1] * x.shape[2] / 8 + 64
+        assert np.all(np.abs(_n(dw) - wsum) <= 2.0 ** -24 * chain * wabs + 2.0 ** -20 * wabs)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-50])  # the second is 0 in fp32
+@pytest.mark.parametrize("dtype,Hq,Hk,D", [("bf16", 1, 2, 128), ("bf16", 12, 5, 128), ("fp32", 4, 9, 64),
+                                           ("fp16", 8, 3, 80), ("bf16", 3, 1, 6)])
+def test_norm_rope_gradients_without_eps(eps, dtype, Hq, Hk, D):
+    """Heads that leave part of a warp's rows empty: those must not reach the weights' sums."""
+    from mlx_primitives.kernels import qk_norm_rope
+    leaves = [t.requires_grad_(True) for t in _norm_case(2, 21, Hq, Hk, D, TYPES[dtype], seed=Hq)]
+    cos, sin = _tables(32, D // 2)
+    pos = np.tile(np.arange(21), (2, 1))
+    pos[1, 13:] = -1
+    out = qk_norm_rope(*leaves, cos, sin, positions=torch.from_numpy(pos).int().cuda(), eps=eps)
+    _check_norm(*leaves, cos, sin, pos, out, 0.0)
+    _check_gradients(leaves, out, pos, cos, sin, 0.0, 5)
