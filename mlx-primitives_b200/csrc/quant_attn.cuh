@@ -464,7 +464,7 @@ __device__ __forceinline__ void qa_step(uint32_t stage, const QaLane<D>& at, con
   uint32_t v[4][Q::VW];
 #pragma unroll
   for (int e = 0; e < 4; ++e) qa_lds<Q::VB>(stage + at.v[e & 1] + (e >> 1) * 8 * D, v[e]);
-  if (masked) {  // rows behind the keys may hold anything
+  if (masked) {  // rows before and behind the keys may hold anything
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -647,6 +647,9 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
     }
     const int k0 = max((r.c0 + ch0) * kQaChunk, r.klo & ~(kQaTile - 1));
     const int k1 = min((long long)(r.c0 + ch1) * kQaChunk, (long long)r.khi);
+    // keys [key_lo, k1): what the first tile holds before a window is as foreign as what lies behind
+    const int key_lo = max(k0, r.klo);
+    const unsigned keys = (unsigned)max(k1 - key_lo, 0);
     const int* bt = p.block_tables + (long long)b * p.bt_stride;
     const long long head_sc = hk * p.sc_sh;
     const float* slope = p.alibi ? s_slope[hp] : nullptr;
@@ -713,10 +716,11 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
           rows.ks0 = rows.ks1 = __shfl_sync(0xffffffffu, cur.ks, i & 31);
           rows.vs0 = rows.vs1 = __shfl_sync(0xffffffffu, cur.vs, i & 31);
           rows.lv0 = rows.lv1 = __shfl_sync(0xffffffffu, cur.lv, i & 31);
-          rows.ok0 = t0 + qa_key(g) < k1;
-          rows.ok1 = t0 + qa_key(g) + 8 < k1;
+          const int from = t0 - key_lo;
+          rows.ok0 = (unsigned)(from + qa_key(g)) < keys;
+          rows.ok1 = (unsigned)(from + qa_key(g) + 8) < keys;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) rows.okv[e] = t0 + c + 4 * e < k1;
+          for (int e = 0; e < 4; ++e) rows.okv[e] = (unsigned)(from + c + 4 * e) < keys;
           qa_step<D, NT, SPLIT, INT8>(ring + stage_out * Q::kTileBytes, at, rows, t0, qf, qs, s_lo, s_hi,
                                       slope, s_pos, t0 < r.flo || t0 + kQaTile > r.fhi, g, c, st);
           stage_out = stage_out + 1 == Q::kStages ? 0 : stage_out + 1;
@@ -747,7 +751,7 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
       const unsigned char* vl = p.v_pool + hk * p.p_sh + Q::VB * qa_piece<D>(g);
       auto locate = [&](int key, long long& off) {
         off = 0;
-        if (key >= k1) return -1;
+        if ((unsigned)(key - key_lo) >= keys) return -1;
         const unsigned slot = (unsigned)key / (unsigned)p.block_size;
         const int got = __ldg(bt + slot);
         if (got < 0 || got >= p.num_blocks) return -1;

@@ -416,27 +416,29 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
       const int* bt = p.block_tables + (long long)u.b * p.bt_stride;
       const long long mine = (long long)u.hk * p.p_sh + rr * p.p_st + 16 * l;  // this lane's piece of row 0
       // A 16-key group of this warp's two in a tile: its pool block and first row's offset, and
-      // how many of its rows are keys.
+      // which of its rows are keys that some query sees (others are not read: their blocks may
+      // have been handed on).
       struct Group {
-        int id, rows;
+        int id;
+        unsigned rows;
         long long off;
       };
       auto group = [&](int j, int g) {
-        Group x{-1, 0, 0};
+        Group x{-1, 0u, 0};
         const int key = (u.r.c0 + j) * kQrKeys + 32 * cw + 16 * g;
-        if (j >= u.ch1 || key >= u.r.khi) return x;
+        if (j >= u.ch1 || key >= u.r.khi || key + 16 <= u.r.klo) return x;
         const unsigned slot = (unsigned)key / (unsigned)p.block_size;
         const int id = __ldg(bt + slot);
         if (id < 0 || id >= p.num_blocks) return x;
         x.id = id;
-        x.rows = min(16, u.r.khi - key);
+        x.rows = 0xffffu >> (16 - min(16, u.r.khi - key)) & 0xffffu << max(0, u.r.klo - key);
         x.off = (long long)id * p.p_sb + (long long)(key - (int)slot * p.block_size) * p.p_st + mine;
         return x;
       };
       auto load = [&](const unsigned char* pool, const Group& g0, const Group& g1, uint4 (&x)[IT]) {
         const unsigned char* q0 = pool + g0.off;
         const unsigned char* q1 = pool + g1.off;
-        if (g0.rows == 16 && g1.rows == 16) {
+        if (g0.rows == 0xffffu && g1.rows == 0xffffu) {
 #pragma unroll
           for (int i = 0; i < IT; ++i)
             x[i] = __ldg(reinterpret_cast<const uint4*>((i < IT / 2 ? q0 : q1) + (i % (IT / 2)) * RPI * p.p_st));
@@ -446,7 +448,7 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
         for (int i = 0; i < IT; ++i) {
           const int k = (i % (IT / 2)) * RPI;  // the piece's row in its group, less rr
           x[i] = make_uint4(0, 0, 0, 0);
-          if (k + rr < (i < IT / 2 ? g0.rows : g1.rows))
+          if ((i < IT / 2 ? g0.rows : g1.rows) >> (k + rr) & 1u)
             x[i] = __ldg(reinterpret_cast<const uint4*>((i < IT / 2 ? q0 : q1) + k * p.p_st));
         }
       };

@@ -7,7 +7,8 @@ import pytest
 import torch
 
 from oracle import cache_oracle as C
-from test_gpu_cache_ops import TYPES, _check_norm, _close, _n, _norm_case, _rand, _tables
+from test_gpu_cache_ops import (TYPES, _attend, _attn_case, _check_attn, _check_norm, _close, _n, _norm_case,
+                                _rand, _tables)
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +42,29 @@ def test_norm_rope_gradients_without_eps(eps, dtype, Hq, Hk, D):
     out = qk_norm_rope(*leaves, cos, sin, positions=torch.from_numpy(pos).int().cuda(), eps=eps)
     _check_norm(*leaves, cos, sin, pos, out, 0.0)
     _check_gradients(leaves, out, pos, cos, sin, 0.0, 5)
+
+
+@pytest.mark.parametrize("Sq", [1, 5, 70, 300])
+@pytest.mark.parametrize("block", [16, 48, 8, 20])
+@pytest.mark.parametrize("window,causal", [(0, True), (5, True), (37, True), (150, False)])
+def test_attention_never_reads_before_the_window(Sq, block, window, causal):
+    """What lies before the first key that any query sees may hold anything: NaN codes in K and V,
+    and scales of NaN where a block holds nothing else."""
+    rs = np.random.RandomState(Sq + block)
+    q, pools, scales, bt, ctx = _attn_case(rs, [1000, 333, Sq + window + 3, 700], 4, 2, 64, block, torch.bfloat16,
+                                           "e4m3", Sq=Sq)
+    stale = np.zeros(pools[0].shape[:2], dtype=bool)
+    for b, n in enumerate(ctx):
+        t = np.arange(max(0, n - Sq - window))
+        stale[bt[b, t // block], t % block] = True
+    stale = torch.from_numpy(stale).cuda()
+    clean = [torch.where(stale[..., None, None], torch.zeros_like(p.view(torch.uint8)), p.view(torch.uint8))
+             .view(p.dtype) for p in pools]
+    csc = [s.clone() for s in scales]
+    for p, s in zip(pools, scales):
+        p.view(torch.uint8)[stale] = 0x7F
+        s[stale.all(1)] = float("nan")
+    kw = dict(window_size=window, causal=causal)
+    out = _attend(q, pools, scales, bt, ctx, **kw)
+    assert torch.isfinite(out).all()
+    _check_attn(out, q, clean, csc, bt, ctx, **kw)
