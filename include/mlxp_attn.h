@@ -451,7 +451,9 @@ int mlxp_paged_append(const mlxp_paged_append_args* args);
  * the query (before it; both sides when not causal).  ALiBi adds slope[h] * (t - position).
  * A query without keys, and rows past query_lens, are zeros.  q and o: fp32, bf16 or fp16, rows
  * 16-byte aligned; pools 16-byte aligned with strides that are multiples of 16; D 32, 64 or 128.
- * Scales are taken as finite, of magnitude 2^-100 to 2^100.  A NaN or infinite value that some row
+ * Scales are taken as finite, K's of magnitude 2^-100 to 2^100.  V's reach to 2^100 and lie within a
+ * factor of 2^80 of one another in a sequence and head; below 2^-60 they count as 2^-60 there, and
+ * the values may count as 0.  A NaN or infinite value that some row
  * of a sequence sees may reach the others of that call.
  */
 typedef struct mlxp_quant_paged_attn_args {

@@ -31,8 +31,10 @@
 // fp16 (bf16 values lose nothing but below 2^-25 of the row's largest); fp32 queries and
 // probabilities are split into two fp16 terms, which keeps 22 bits.  The running maximum m is of
 // s_t + log2 |vs_t|, so that the weights p_t vs_t 2^15 that multiply V8 fit fp16 whatever the
-// scales, with 29 octaves below the largest at full precision; m and the sums are fp32.  |vs_t|
-// is taken as within [2^-100, 2^100] there.
+// scales, with 29 octaves below the largest at full precision; m and the sums are fp32.  V's
+// scales are taken as at most 2^100, and within 2^80 of each other in a sequence and head, those
+// below 2^-60 counting as that: keys of 2^-46 of the largest weight and more are then never lost
+// from the sum, whose factors are fp32 powers of two down to 2^-126.
 //
 // Work split.  A virtual sequence is a sequence and a tile of 8 NT of its G * Sq query rows; it
 // has Hk / HP units, HP heads each: the warps of a CTA take HP heads (reading neighbouring bytes
@@ -356,8 +358,13 @@ struct QaRows {
   bool ok0, ok1, okv[4];
 };
 
+// log2 |vs| as the running maximum takes it.  Scales below 2^-60 (blocks of zero values have 2^-126)
+// count as 2^-60 there: the sum of the weights without vs is rescaled along with the maximum, and
+// a factor below 2^-126 would be 0 and take keys out of it that do have weight.
+constexpr float kQaLeastLog = -60.f, kQaLeastScale = 0x1p-60f;
+
 __device__ __forceinline__ float qa_log_scale(float vs) {
-  return fminf(fmaxf(__log2f(fabsf(vs)), -100.f), 100.f);
+  return fminf(fmaxf(__log2f(fabsf(vs)), kQaLeastLog), 100.f);
 }
 
 template <int D, int NT, bool SPLIT, bool INT8>

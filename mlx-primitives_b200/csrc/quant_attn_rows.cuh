@@ -15,7 +15,7 @@
 // the operands: K's multiply the scores' columns (one factor a 16-key group, the block size being
 // a multiple of 16), V's the weights, as a term of their exponent.  Negative scales' signs move
 // into the codes, so that a group's maximum is its scores' maximum times the scale and the
-// exponent has a logarithm to add.
+// exponent has a logarithm to add; values whose scale is below the least logarithm are zeros.
 //
 // Roles, 12 warps: two softmax warpgroups, a thread a row (scores from TMEM into registers,
 // weights back over them as fp16), whose first thread also issues its tile's MMAs,
@@ -415,30 +415,38 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
       const Unit u = next_unit();
       const int* bt = p.block_tables + (long long)u.b * p.bt_stride;
       const long long mine = (long long)u.hk * p.p_sh + rr * p.p_st + 16 * l;  // this lane's piece of row 0
-      // A 16-key group of this warp's two in a tile: its pool block and first row's offset, and
-      // which of its rows are keys that some query sees (others are not read: their blocks may
-      // have been handed on).
+      // A 16-key group of this warp's two in a tile: its first row's offset, and which of its rows
+      // are keys that some query sees (others are not read: their blocks may have been handed on);
+      // none where it has no block.
       struct Group {
-        int id;
         unsigned rows;
         long long off;
       };
-      auto group = [&](int j, int g) {
-        Group x{-1, 0u, 0};
-        const int key = (u.r.c0 + j) * kQrKeys + 32 * cw + 16 * g;
-        if (j >= u.ch1 || key >= u.r.khi || key + 16 <= u.r.klo) return x;
-        const unsigned slot = (unsigned)key / (unsigned)p.block_size;
-        const int id = __ldg(bt + slot);
-        if (id < 0 || id >= p.num_blocks) return x;
-        x.id = id;
-        x.rows = 0xffffu >> (16 - min(16, u.r.khi - key)) & 0xffffu << max(0, u.r.klo - key);
-        x.off = (long long)id * p.p_sb + (long long)(key - (int)slot * p.block_size) * p.p_st + mine;
-        return x;
+      // Groups 0 and 1 of tile j; lane i holds the scales of group i & 1.
+      auto groups = [&](int j, Group& g0, Group& g1, float& ks, float& vs) {
+        ks = vs = 0.f;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          Group& x = g ? g1 : g0;
+          x = Group{0u, 0};
+          const int key = (u.r.c0 + j) * kQrKeys + 32 * cw + 16 * g;
+          if (j >= u.ch1 || key >= u.r.khi || key + 16 <= u.r.klo) continue;
+          const unsigned slot = (unsigned)key / (unsigned)p.block_size;
+          const int id = __ldg(bt + slot);
+          if (id < 0 || id >= p.num_blocks) continue;
+          x.rows = 0xffffu >> (16 - min(16, u.r.khi - key)) & 0xffffu << max(0, u.r.klo - key);
+          x.off = (long long)id * p.p_sb + (long long)(key - (int)slot * p.block_size) * p.p_st + mine;
+          if ((lane & 1) == g) {
+            const long long at = (long long)id * p.sc_sb + (long long)u.hk * p.sc_sh;
+            ks = __ldg(p.k_scales + at);
+            vs = __ldg(p.v_scales + at);
+          }
+        }
       };
       auto load = [&](const unsigned char* pool, const Group& g0, const Group& g1, uint4 (&x)[IT]) {
         const unsigned char* q0 = pool + g0.off;
         const unsigned char* q1 = pool + g1.off;
-        if (g0.rows == 0xffffu && g1.rows == 0xffffu) {
+        if ((g0.rows & g1.rows) == 0xffffu) {
 #pragma unroll
           for (int i = 0; i < IT; ++i)
             x[i] = __ldg(reinterpret_cast<const uint4*>((i < IT / 2 ? q0 : q1) + (i % (IT / 2)) * RPI * p.p_st));
@@ -452,26 +460,23 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
             x[i] = __ldg(reinterpret_cast<const uint4*>((i < IT / 2 ? q0 : q1) + k * p.p_st));
         }
       };
-      // lanes 0 and 1 hold the scales of the two groups
-      auto scales = [&](const Group& g0, const Group& g1, float& ks, float& vs) {
-        const int id = lane == 0 ? g0.id : lane == 1 ? g1.id : -1;
-        ks = vs = 0.f;
-        if (id < 0) return;
-        const long long at = (long long)id * p.sc_sb + (long long)u.hk * p.sc_sh;
-        ks = __ldg(p.k_scales + at);
-        vs = __ldg(p.v_scales + at);
+      // V's codes where their scale counts (scale: as the lanes hold it), else zeros.
+      auto load_v = [&](Group g0, Group g1, float scale, uint4 (&x)[IT]) {
+        const uint32_t none = __ballot_sync(0xffffffffu, fabsf(scale) < kQaLeastScale);
+        if (none & 1u) g0.rows = 0u;
+        if (none & 2u) g1.rows = 0u;
+        load(p.v_pool, g0, g1, x);
       };
-      Group a0 = group(u.ch0, 0), a1 = group(u.ch0, 1);  // of tile j, and of j + 1
-      Group b0 = group(u.ch0 + 1, 0), b1 = group(u.ch0 + 1, 1);
+      Group a0, a1, b0, b1;  // of tile j, and of j + 1
       uint4 kx[IT], vx[IT];
       float ks, vs, ks_next, vs_next;
+      groups(u.ch0, a0, a1, ks, vs);
       load(p.k_pool, a0, a1, kx);
-      load(p.v_pool, a0, a1, vx);
-      scales(a0, a1, ks, vs);
+      load_v(a0, a1, vs, vx);
+      groups(u.ch0 + 1, b0, b1, ks_next, vs_next);
       bool ok = true;
       for (int j = u.ch0; j < u.ch1; ++j) {
         const int c = cnt + j - u.ch0, st = c & 1;
-        scales(b0, b1, ks_next, vs_next);
         const uint32_t k_neg = __ballot_sync(0xffffffffu, ks < 0.f);
         const uint32_t v_neg = __ballot_sync(0xffffffffu, vs < 0.f);
         if (c >= 2) {
@@ -483,7 +488,7 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
               make_float4(fmaxf(fabsf(ks), 7.5e-37f), qa_log_scale(vs), ex2_approx(-qa_log_scale(vs)), 0.f);
         }
         if (lane == 2)
-          (smem + C::OFF_MASK)[(c & 3) * 4 + cw] = (unsigned char)((a0.id >= 0) | (a1.id >= 0) << 1);
+          (smem + C::OFF_MASK)[(c & 3) * 4 + cw] = (unsigned char)((a0.rows != 0u) | (a1.rows != 0u) << 1);
         const uint32_t kt = sbase + C::OFF_K + st * C::TILE;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
@@ -505,13 +510,12 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(BAR(C::B_VF + st));
-        load(p.v_pool, b0, b1, vx);
+        load_v(b0, b1, vs_next, vx);
         a0 = b0;
         a1 = b1;
-        b0 = group(j + 2, 0);
-        b1 = group(j + 2, 1);
         ks = ks_next;
         vs = vs_next;
+        groups(j + 2, b0, b1, ks_next, vs_next);
       }
       cnt += u.ch1 - u.ch0;
       if (!ok) break;

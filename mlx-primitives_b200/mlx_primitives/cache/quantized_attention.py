@@ -51,7 +51,9 @@ def quantized_paged_attention(
 
     k_pool, v_pool: (num_blocks, block_size, kv_heads, head_dim) float8_e4m3fn or int8, heads a
     multiple of kv_heads, 16-byte aligned with strides that are multiples of 16; k_scales,
-    v_scales: (num_blocks, kv_heads) float32, finite, of magnitude 2^-100 to 2^100.  block_tables:
+    v_scales: (num_blocks, kv_heads) float32, finite, k's of magnitude 2^-100 to 2^100, v's to 2^100
+    and within a factor of 2^80 of one another in a sequence and head (below 2^-60, as blocks of
+    zeros have it, they count as 2^-60 there and the values may count as 0).  block_tables:
     (batch, max_blocks), ids outside [0, num_blocks) are missing blocks.  context_lens: (batch,)
     cached tokens, the queries' own among them.  ``query_lens`` (batch,): queries of each sequence
     (default seq_q); rows behind them come back as zeros, as do rows that see no key.

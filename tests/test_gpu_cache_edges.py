@@ -2,6 +2,8 @@
 their scales, masks and sizes, autograd's other modes, and the ways a call can take to the kernels.
 Tolerances are those of that file, which derives them."""
 
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -68,3 +70,50 @@ def test_attention_never_reads_before_the_window(Sq, block, window, causal):
     out = _attend(q, pools, scales, bt, ctx, **kw)
     assert torch.isfinite(out).all()
     _check_attn(out, q, clean, csc, bt, ctx, **kw)
+
+
+@pytest.mark.parametrize("Sq", [1, 3, 70])
+@pytest.mark.parametrize("zeros", [2.0 ** -126, 0.0])
+def test_attention_blocks_of_zero_values_count(Sq, zeros):
+    """Blocks whose values are all zero, as paged_append writes them (scale 2^-126), weigh in the
+    softmax like any other, before and behind the others, in one CTA and in many."""
+    for blocks, dtype in ((65, torch.bfloat16), (65, torch.float32), (1300, torch.float16)):
+        for last in (True, False):
+            bt = np.arange(blocks, dtype=np.int32)[None]
+            big = blocks - 1 if last else 0
+            shape = (blocks, 16, 1, 64)
+            k, v = torch.zeros(shape, device="cuda"), torch.zeros(shape, device="cuda")
+            k[..., 0] = -8.0  # scores of 2^-8 in the softmax's base below
+            k[big] = 0.0
+            v[big] = 1.0
+            pools = [t.to(torch.float8_e4m3fn) for t in (k, v)]
+            size = 2.0 ** 10 if dtype is torch.float16 else 2.0 ** 20
+            scales = [torch.ones(blocks, 1, device="cuda"), torch.full((blocks, 1), zeros, device="cuda")]
+            scales[1][big] = size
+            q = torch.zeros(1, Sq, 1, 64, dtype=dtype, device="cuda")
+            q[..., 0] = 1.0
+            out = _attend(q, pools, scales, bt, np.array([16 * blocks], dtype=np.int32), scale=math.log(2.0),
+                          causal=False)
+            want = np.full(q.shape, size * 16 / (16 + 16 * (blocks - 1) * 2.0 ** -8))
+            # two different weights a row and one value: the weights' fp16 rounding, and the sums
+            _close(out, want, dtype, (2.0 ** -15 if dtype is torch.float32 else 2.0 ** -11 + 2.0 ** -14) * want)
+    scales[1].zero_()
+    pools[1].view(torch.uint8).fill_(0x38)
+    assert torch.all(_attend(q.bfloat16(), pools, scales, bt, np.array([16 * blocks], dtype=np.int32)) == 0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("Sq", [1, 5, 70])
+def test_attention_value_scales_at_their_limits(dtype, Sq):
+    """Scales of values 2^80 apart, block by block and in stretches longer than a CTA's."""
+    rs = np.random.RandomState(41)
+    case = _attn_case(rs, [2000, 130, 9000], 4, 2, 64, 16, TYPES[dtype], "e4m3", Sq=Sq, qsize=0.5)
+    q, pools, scales, bt, ctx = case
+    for stretch in (1, 9, 200):
+        small = (np.arange(scales[1].shape[0]) // stretch % 2).astype(bool)
+        order = np.concatenate([bt[b, :-(-n // 16)] for b, n in enumerate(ctx)])
+        for lo, hi in ((2.0 ** -60, 2.0 ** 20), (2.0 ** 20, 2.0 ** 100)):
+            vs = np.ones(scales[1].shape[0])
+            vs[order] = np.where(small[:order.size], lo, hi)
+            scales[1].copy_(torch.from_numpy(vs)[:, None])
+            _check_attn(_attend(*case), *case)
