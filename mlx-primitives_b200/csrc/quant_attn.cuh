@@ -27,7 +27,7 @@
 // V row the eight lanes g hold D / 8 bytes each, and a byte permute of two keys' words gives the
 // pairs along keys.
 //
-// Precision.  16-bit queries are scaled by a power of two a row to [1, 2) at most and held in
+// Precision.  16-bit queries are scaled by a power of two a row to below 4 and held in
 // fp16 (bf16 values lose nothing but below 2^-25 of the row's largest); fp32 queries and
 // probabilities are split into two fp16 terms, which keeps 22 bits.  The running maximum m is of
 // s_t + log2 |vs_t|, so that the weights p_t vs_t 2^15 that multiply V8 fit fp16 whatever the
@@ -529,7 +529,7 @@ __device__ __forceinline__ void qa_load_q(const QaParams& p, int b, int r0, int 
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const unsigned E = __float_as_uint(mx) >> 23;
-      if (E >= 1 && E <= 253) up = __uint_as_float(E << 23);
+      if (E >= 1 && E <= 254) up = __uint_as_float(min(E, 253u) << 23);  // its inverse is not 0
       const float down = __uint_as_float((254u - (__float_as_uint(up) >> 23)) << 23);
 #pragma unroll
       for (int e = 0; e < D / 4; ++e) x[e] *= down;

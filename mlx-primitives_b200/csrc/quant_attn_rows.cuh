@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
 #pragma unroll
             for (int off = 1; off < QL; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
             const unsigned E = __float_as_uint(mx) >> 23;
-            const unsigned up = E >= 1 && E <= 253 ? E : 127u;  // the row is below 2^(up - 126)
+            const unsigned up = E >= 1 && E <= 254 ? min(E, 253u) : 127u;  // 2^-up is not 0
             const float down = __uint_as_float((254u - up) << 23);
 #pragma unroll
             for (int e = 0; e < 4; ++e)

@@ -117,3 +117,15 @@ def test_attention_value_scales_at_their_limits(dtype, Sq):
             vs[order] = np.where(small[:order.size], lo, hi)
             scales[1].copy_(torch.from_numpy(vs)[:, None])
             _check_attn(_attend(*case), *case)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("Sq", [1, 3, 70])
+def test_attention_queries_near_the_largest_value(dtype, Sq):
+    rs = np.random.RandomState(42)
+    case = _attn_case(rs, [300, 90], 4, 2, 64, 16, TYPES[dtype], "e4m3", Sq=Sq)
+    q, pools, scales, bt, ctx = case
+    q.copy_(q.clamp(-4, 4) / 4 * 3e38)
+    q[..., 0] = 2.0 ** 127
+    scales[0].mul_(2.0 ** -90)  # scores of a few, once multiplied by 2^-36
+    _check_attn(_attend(*case, scale=2.0 ** -36), *case, scale=2.0 ** -36)
