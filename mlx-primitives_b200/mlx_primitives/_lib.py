@@ -144,6 +144,8 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_WIDE_INTS = (torch.int64, torch.uint32, torch.uint64)
+
 _calls = None
 
 
@@ -170,6 +172,14 @@ def rows_like(x: torch.Tensor) -> torch.Tensor:
     unfolded view), empty_like may order the dimensions otherwise."""
     t = torch.empty_like(x)
     return t if t.stride(-1) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def int32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """Integers as int32 on `device`.  What 32 bits do not hold becomes the nearest that they do,
+    which is no block, row or position either (cut to its low bits it could be one)."""
+    if t.dtype in _WIDE_INTS:
+        t = t.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1)
+    return t.to(device, torch.int32)
 
 
 def last_error() -> str:

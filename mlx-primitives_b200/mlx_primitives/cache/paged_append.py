@@ -66,7 +66,7 @@ def device_ints(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
     if t.dtype is not torch.int32 or t.get_device() != like.get_device():
         if t.is_floating_point():
             raise ValueError(f"block tables and lengths must be integers, got {t.dtype}")
-        t = t.to(like.device, torch.int32)
+        t = _lib.int32(t, like.device)
     return t if t.is_contiguous() or t.stride(-1) == 1 else t.contiguous()
 
 

@@ -212,7 +212,7 @@ def qk_norm_rope(
         if not _lib.plain(sin_cache, dev, torch.float32):
             sin_cache = sin_cache.detach().to(q.device, torch.float32).contiguous()
     if positions is not None and (positions.dtype is not torch.int32 or positions.get_device() != dev):
-        positions = positions.to(q.device, torch.int32)
+        positions = _lib.int32(positions, q.device)
     offset = int(offset)
     k_offset = offset if k_offset is None else int(k_offset)
     run = _QKNormRopeFn.apply if needs else _forward

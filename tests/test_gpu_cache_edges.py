@@ -129,3 +129,38 @@ def test_attention_queries_near_the_largest_value(dtype, Sq):
     q[..., 0] = 2.0 ** 127
     scales[0].mul_(2.0 ** -90)  # scores of a few, once multiplied by 2^-36
     _check_attn(_attend(*case, scale=2.0 ** -36), *case, scale=2.0 ** -36)
+
+
+def test_integers_past_32_bits():
+    """64-bit lengths, tables and positions are not cut: 2^32 + 1 is no block and no row."""
+    from mlx_primitives.cache import paged_append, quantized_paged_attention
+    from mlx_primitives.kernels import qk_norm_rope
+    rs = np.random.RandomState(48)
+    far = 1 << 32
+    q, k, qw, kw = _norm_case(1, 4, 4, 2, 64, torch.bfloat16)
+    cos, sin = _tables(8, 32)
+    pos = np.array([[far + 1, 3, -far, far * 2 - 1]])
+    out = qk_norm_rope(q, k, qw, kw, cos, sin, positions=torch.from_numpy(pos).cuda())
+    _check_norm(q, k, qw, kw, cos, sin, pos, out)
+    qa, pools, scales, bt, ctx = _attn_case(rs, [300, 90], 4, 2, 64, 16, torch.bfloat16, "e4m3")
+    holes = bt.copy()
+    holes[0, 3], holes[1, 0] = -1, -1
+    far_bt = bt.astype(np.int64)
+    far_bt[0, 3], far_bt[1, 0] = far + int(bt[0, 3]), -far + int(bt[1, 0])
+    want = _attend(qa, pools, scales, holes, ctx)
+    assert torch.equal(_attend(qa, pools, scales, far_bt, ctx), want)
+    lens = np.array([far + 5, -far + 40])
+    assert torch.equal(_attend(qa, pools, scales, bt, lens),
+                       _attend(qa, pools, scales, bt, np.array([2 ** 31 - 1, 0], dtype=np.int32)))
+    x = _rand(rs, (2, 1, 2, 64), torch.bfloat16)
+    before = [t.view(torch.uint8).clone() for t in pools]
+    paged_append(x, x, *pools, torch.from_numpy(bt).cuda(), torch.from_numpy(lens).cuda(), k_scales=scales[0],
+                 v_scales=scales[1])
+    paged_append(x, x, *pools, torch.from_numpy(far_bt).cuda(), torch.tensor([50, 2]).cuda(), k_scales=scales[0],
+                 v_scales=scales[1])
+    for a, b in zip(pools, before):
+        assert torch.equal(a.view(torch.uint8), b)
+    paged_append(x, x, *pools, torch.from_numpy(bt).cuda(), torch.tensor([5, 5]).cuda(),
+                 new_lens=torch.tensor([far, -far]).cuda(), k_scales=scales[0], v_scales=scales[1])
+    same = [torch.equal(p.view(torch.uint8)[bt[b, 0]], w[bt[b, 0]]) for p, w in zip(pools, before) for b in range(2)]
+    assert same == [False, True, False, True]
