@@ -62,12 +62,15 @@ def check_pools(k_pool, v_pool, k_scales, v_scales):
 
 
 def device_ints(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
-    """Tables and lengths as the kernels read them: int32 beside `like`, unit inner stride."""
+    """Tables and lengths as the kernels read them: int32 beside `like`, unit inner stride, rows that
+    do not overlap (one table expanded over the batch is copied)."""
     if t.dtype is not torch.int32 or t.get_device() != like.get_device():
         if t.is_floating_point():
             raise ValueError(f"block tables and lengths must be integers, got {t.dtype}")
         t = _lib.int32(t, like.device)
-    return t if t.is_contiguous() or t.stride(-1) == 1 else t.contiguous()
+    if t.is_contiguous() or (t.stride(-1) == 1 and (t.ndim < 2 or t.stride(0) >= t.shape[1])):
+        return t
+    return t.contiguous()
 
 
 def paged_append(

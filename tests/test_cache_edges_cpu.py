@@ -16,3 +16,17 @@ def test_integers_are_cut_to_their_nearest(dtype):
     got = _lib.int32(t, torch.device("cpu"))
     assert got.dtype is torch.int32 and got.tolist() == [min(max(v, low), top) for v in values]
     assert torch.equal(t, was)
+
+
+def test_tables_and_lengths_as_the_kernels_read_them():
+    from mlx_primitives.cache.paged_append import device_ints
+    like = torch.zeros(1)
+    one = torch.arange(5, dtype=torch.int32)[None]
+    for t in (one, one.repeat(3, 1), torch.arange(24, dtype=torch.int32).view(3, 8)[:, :5], one.expand(1, 5)):
+        assert device_ints(t, like) is t
+    for t in (one.expand(3, 5), torch.arange(10, dtype=torch.int32).as_strided((3, 5), (2, 1)),
+              torch.arange(15, dtype=torch.int32).view(5, 3).T, one[0, :1].expand(4)):
+        got = device_ints(t, like)
+        assert got.is_contiguous() and torch.equal(got, t)
+    with pytest.raises(ValueError, match="integers"):
+        device_ints(one.float(), like)

@@ -131,6 +131,27 @@ def test_attention_queries_near_the_largest_value(dtype, Sq):
     _check_attn(_attend(*case, scale=2.0 ** -36), *case, scale=2.0 ** -36)
 
 
+def test_block_tables_shared_by_expansion():
+    """One table for all sequences, as a view without a row stride."""
+    from mlx_primitives.cache import paged_append, quantized_paged_attention
+    rs = np.random.RandomState(47)
+    q, pools, scales, bt, ctx = _attn_case(rs, [300], 4, 2, 64, 16, torch.bfloat16, "e4m3")
+    one = torch.from_numpy(bt).cuda()
+    qs = _rand(rs, (3, 1, 4, 64), torch.bfloat16, 2.0)
+    lens = torch.tensor([300, 17, 120], dtype=torch.int32, device="cuda")
+    for t in (one, one.long()):
+        got = quantized_paged_attention(qs, *pools, *scales, t.expand(3, -1), lens)
+        assert torch.equal(got, quantized_paged_attention(qs, *pools, *scales, t.repeat(3, 1), lens))
+    k = _rand(rs, (3, 2, 2, 64), torch.bfloat16)
+    new = torch.tensor([2, 0, 0], dtype=torch.int32, device="cuda")  # one writer of the shared block
+    both = [[t.clone() for t in (*pools, *scales)] for _ in range(2)]
+    for t, table in zip(both, (one.expand(3, -1), one.repeat(3, 1))):
+        paged_append(k, k, t[0], t[1], table, lens, new_lens=new, k_scales=t[2], v_scales=t[3])
+    for a, b in zip(*both):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert not torch.equal(both[0][0].view(torch.uint8), pools[0].view(torch.uint8))
+
+
 def test_integers_past_32_bits():
     """64-bit lengths, tables and positions are not cut: 2^32 + 1 is no block and no row."""
     from mlx_primitives.cache import paged_append, quantized_paged_attention
