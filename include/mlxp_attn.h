@@ -418,6 +418,7 @@ size_t mlxp_qk_norm_rope_bwd_workspace_size(int64_t D);
  * and its earlier codes are rescaled.  Codes are round-to-nearest-even of value / scale, clamped
  * to +-qmax; NaN stays NaN in e4m3 and is 0 in int8.
  *
+ * max_blocks * block_size is at most 2^31 - 1024.
  * A block that receives tokens must be listed once: sequences may share only blocks that are full.
  * k_pool and v_pool (and the scales) are different memory.
  */
@@ -451,6 +452,7 @@ int mlxp_paged_append(const mlxp_paged_append_args* args);
  * the query (before it; both sides when not causal).  ALiBi adds slope[h] * (t - position).
  * A query without keys, and rows past query_lens, are zeros.  q and o: fp32, bf16 or fp16, rows
  * 16-byte aligned; pools 16-byte aligned with strides that are multiples of 16; D 32, 64 or 128.
+ * max_blocks * block_size and B * Sq * H are at most 2^31 - 1024.
  * Scales are taken as finite, K's of magnitude 2^-100 to 2^100.  V's reach to 2^100 and lie within a
  * factor of 2^80 of one another in a sequence and head; below 2^-60 they count as 2^-60 there, and
  * the values may count as 0.  A NaN or infinite value that some row

@@ -10,6 +10,10 @@
 
 namespace mlxp {
 
+// Positions a sequence's block table may reach, and query rows a call may have, in the cache
+// kernels, whose indexes are 32-bit: room for a few tiles past the last one.
+constexpr long long kMaxCacheIndex = 0x7fffffffLL - 1023;
+
 // Records the message of mlxp_last_error and returns `code`.
 MLXP_INTERNAL int fail(int code, const char* fmt, ...);
 MLXP_INTERNAL int cuda_fail(cudaError_t e, const char* what);

@@ -286,7 +286,7 @@ int mlxp_paged_append(const mlxp_paged_append_args* a) {
     if (int rc = check_dtype(a->k_weight_dtype, "k_weight")) return rc;
   if (!(a->eps >= 0) || !std::isfinite(a->eps)) return fail(MLXP_ERR_INVALID, "eps must be finite and >= 0");
   if (a->num_blocks > INT32_MAX || a->block_size > INT32_MAX || a->max_blocks > INT32_MAX ||
-      a->max_blocks * a->block_size > INT32_MAX || a->B > INT32_MAX || a->S > INT32_MAX ||
+      a->max_blocks * a->block_size > kMaxCacheIndex || a->B > INT32_MAX || a->S > INT32_MAX ||
       a->B * a->S > INT32_MAX || a->B * a->S * std::max(a->q ? a->Hq : 1, a->Hk) > INT32_MAX)
     return fail(MLXP_ERR_INVALID, "paged shape too large");
   if (a->B == 0 || a->S == 0) return MLXP_OK;

@@ -72,8 +72,8 @@ int qa_check(const mlxp_quant_paged_attn_args* a) {
     return fail(MLXP_ERR_UNSUPPORTED, "paged attention supports head_dim 32, 64 and 128, got %lld",
                 (long long)a->D);
   if (a->num_blocks > INT32_MAX || a->block_size > INT32_MAX || a->max_blocks > INT32_MAX ||
-      a->max_blocks * a->block_size > INT32_MAX || a->B > INT32_MAX || a->Sq > INT32_MAX ||
-      a->H > INT32_MAX || a->B * a->Sq > INT32_MAX || a->B * a->Sq * a->H > INT32_MAX)
+      a->max_blocks * a->block_size > kMaxCacheIndex || a->B > INT32_MAX || a->Sq > INT32_MAX ||
+      a->H > INT32_MAX || a->B * a->Sq > INT32_MAX || a->B * a->Sq * a->H > kMaxCacheIndex)
     return fail(MLXP_ERR_INVALID, "paged shape too large");
   if (a->window < -1) return fail(MLXP_ERR_INVALID, "window must be >= 0, or -1 for none");
   return MLXP_OK;

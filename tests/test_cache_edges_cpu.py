@@ -30,3 +30,32 @@ def test_tables_and_lengths_as_the_kernels_read_them():
         assert got.is_contiguous() and torch.equal(got, t)
     with pytest.raises(ValueError, match="integers"):
         device_ints(one.float(), like)
+
+
+def test_sizes_that_32_bit_indexes_do_not_hold_are_refused():
+    """Up to a thousand below 2^31: the kernels count a few tiles past the last key or row."""
+    from mlx_primitives import _lib
+    from mlx_primitives.cache.paged_append import _ARGS as APPEND
+    from mlx_primitives.cache.quantized_attention import _ARGS as ATTN
+    L, top = _lib.lib(), (1 << 31) - 1
+
+    def append(block, mb, v_pool=32):
+        return L.mlxp_paged_append(APPEND.pack(
+            16, 16, 0, 0, 16, v_pool, 0, 0, 16, 16, 0, 0, 0, 0, 0, 1, 1, 0, 0, 1, 1, 0, 1, 64, 8, block, mb, mb, 0,
+            *[64] * 12, *[64] * 3, 1, 1, 1e-6, 0))
+
+    def attn(block, mb, B=1, Sq=1, H=4, scale=0.1):
+        return L.mlxp_quant_paged_attn(ATTN.pack(
+            16, 16, 16, 16, 16, 16, 16, 16, 0, 0, 1, 3, B, Sq, H, 2, 64, 8, block, mb, mb, 1, -1, 64, 64, 64, 64, 64,
+            64, 64, 64, 64, 2, 1, scale, 0, 0, 0))
+
+    for call in (lambda: append(top, 1), lambda: append(1, top - 1022), lambda: append(16, (top >> 4) - 62),
+                 lambda: attn(top, 1), lambda: attn(1, top - 1022), lambda: attn(16, (top >> 4) - 62),
+                 lambda: attn(16, 4, B=1 << 19, Sq=1 << 10), lambda: attn(16, 4, Sq=(top >> 2) - 254)):
+        assert call() == _lib.MLXP_ERR_INVALID
+        assert b"too large" in L.mlxp_last_error()
+    # the largest that are taken: refused for another reason, which is looked at behind the sizes
+    assert append(1, top - 1023, v_pool=16) == _lib.MLXP_ERR_INVALID
+    assert b"different" in L.mlxp_last_error()
+    assert attn(1, top - 1023, Sq=(top >> 2) - 255, scale=0.0) == _lib.MLXP_ERR_INVALID
+    assert b"scale" in L.mlxp_last_error()
