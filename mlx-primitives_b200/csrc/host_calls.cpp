@@ -343,8 +343,9 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if ((qw && (!q || !weight(qw, dev, D))) || (kw && !weight(kw, dev, D)) || bool(c) != bool(s)) return none();
     if (c && !(table(c, dev, D / 2) && table(s, dev, D / 2) && c->size(0) == s->size(0) && c->size(0) >= mb * block))
       return none();
-    if (at::GradMode::is_enabled() && (wants_grad(k) || wants_grad(v) || wants_grad(q) || wants_grad(qw) || wants_grad(kw)))
-      return none();
+    if (at::GradMode::is_enabled())
+      for (const Arg* x : {&k, &v, &q, &qw, &kw, &kp, &vp, &ks, &vs})
+        if (wants_grad(*x)) return none();
     mlxp_paged_append_args x{};
     x.size = sizeof(x);
     at::Tensor qo;
@@ -417,7 +418,9 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (bt->scalar_type() != at::kInt || !on(bt, dev) || bt->dim() != 2 || bt->size(0) != B || !bt->is_contiguous() ||
         !ints(ctx, dev, B) || (lens && !ints(lens, dev, B)))
       return none();
-    if (at::GradMode::is_enabled() && wants_grad(q)) return none();
+    if (at::GradMode::is_enabled())
+      for (const Arg* x : {&q, &kp, &vp, &ks, &vs})
+        if (wants_grad(*x)) return none();
     at::Tensor o = at::empty_like(*q.t);
     mlxp_quant_paged_attn_args x{};
     x.size = sizeof(x);

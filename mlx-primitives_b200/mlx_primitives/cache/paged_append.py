@@ -61,6 +61,12 @@ def check_pools(k_pool, v_pool, k_scales, v_scales):
     return code
 
 
+def refuse_gradients(what, *tensors):
+    """Raises where a call without derivatives is given tensors that want one."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError(f"{what} is not differentiable: call it under torch.no_grad()")
+
+
 def device_ints(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
     """Tables and lengths as the kernels read them: int32 beside `like`, unit inner stride, rows that
     do not overlap (one table expanded over the batch is copied)."""
@@ -134,6 +140,7 @@ def paged_append(
         raise ValueError(f"pools of (heads, head_dim) = {(Hp, Dp)} cannot take k of {(Hk, D)}")
     if D % 2 or D < 2:
         raise ValueError(f"head_dim must be even, got {D}")
+    refuse_gradients("paged_append", k, v, q, k_pool, v_pool, k_scales, v_scales, q_weight, k_weight)
     dev = k.get_device()
     if dev < 0 or k_pool.get_device() != dev or v_pool.get_device() != dev or v.get_device() != dev:
         raise ValueError("k, v and the pools must be on one CUDA device (appending is in place)")
@@ -146,9 +153,6 @@ def paged_append(
     if context_lens.shape != (B,) or (new_lens is not None and new_lens.shape != (B,)):
         raise ValueError(f"context_lens and new_lens must be (batch,) = ({B},), got "
                          f"{tuple(context_lens.shape)} and {None if new_lens is None else tuple(new_lens.shape)}")
-    grad = torch.is_grad_enabled()
-    if grad and (k.requires_grad or v.requires_grad):
-        _no_gradients()
     q_ptr = qo_ptr = Hq = 0
     qs = qo = (0, 0, 0, 1)
     q_out = None
@@ -157,8 +161,6 @@ def paged_append(
         if (len(q_shape) != 4 or q_shape[0] != B or q_shape[1] != S or q_shape[3] != D
                 or q.dtype is not dtype or q.get_device() != dev):
             raise ValueError(f"q must be ({B}, {S}, heads, {D}) {dtype} beside k, got {tuple(q.shape)} {q.dtype}")
-        if grad and q.requires_grad:
-            _no_gradients()
         Hq = q_shape[2]
         qs = q.stride()
         if qs[3] != 1:
@@ -170,10 +172,10 @@ def paged_append(
         raise ValueError("q_weight needs q")
     qw_ptr = kw_ptr = qw_code = kw_code = 0
     if q_weight is not None:
-        q_weight = _weight("q_weight", q_weight, D, k, grad)
+        q_weight = _weight("q_weight", q_weight, D, k)
         qw_ptr, qw_code = q_weight.data_ptr(), codes[q_weight.dtype]
     if k_weight is not None:
-        k_weight = _weight("k_weight", k_weight, D, k, grad)
+        k_weight = _weight("k_weight", k_weight, D, k)
         kw_ptr, kw_code = k_weight.data_ptr(), codes[k_weight.dtype]
     if (cos_cache is None) != (sin_cache is None):
         raise ValueError("cos_cache and sin_cache must be given together")
@@ -221,13 +223,7 @@ def paged_append(
     return q_out
 
 
-def _no_gradients():
-    raise NotImplementedError("paged_append is not differentiable: call it under torch.no_grad()")
-
-
-def _weight(name, w, D, k, grad):
+def _weight(name, w, D, k):
     if w.shape != (D,) or w.dtype not in _lib.DTYPE_CODES:
         raise ValueError(f"{name} must be ({D},) of a supported dtype, got {tuple(w.shape)} {w.dtype}")
-    if grad and w.requires_grad:
-        _no_gradients()
     return w if _lib.plain(w, k.get_device(), w.dtype) else w.to(k.device).contiguous()

@@ -18,7 +18,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .paged_append import check_pools, device_ints
+from .paged_append import check_pools, device_ints, refuse_gradients
 
 __all__ = ["quantized_paged_attention"]
 
@@ -99,9 +99,7 @@ def quantized_paged_attention(
         raise ValueError(f"alibi_slopes must be (num_heads,) = ({H},), got {tuple(alibi_slopes.shape)}")
     if window_size is not None and window_size < 0:
         raise ValueError(f"window_size must be >= 0, got {window_size}")
-    if q.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError("quantized_paged_attention is not differentiable: call it under "
-                                  "torch.no_grad()")
+    refuse_gradients("quantized_paged_attention", q, k_pool, v_pool, k_scales, v_scales, alibi_slopes)
     dev = q.get_device()
     host = dev < 0
     if host:

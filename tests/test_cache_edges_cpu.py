@@ -59,3 +59,31 @@ def test_sizes_that_32_bit_indexes_do_not_hold_are_refused():
     assert b"different" in L.mlxp_last_error()
     assert attn(1, top - 1023, Sq=(top >> 2) - 255, scale=0.0) == _lib.MLXP_ERR_INVALID
     assert b"scale" in L.mlxp_last_error()
+
+
+def _pool_args(dtype=torch.float32):
+    z = lambda *shape: torch.zeros(shape)
+    i = lambda *shape: torch.zeros(shape, dtype=torch.int32)
+    return z(1, 1, 2, 64), z(3, 16, 2, 64).to(dtype), i(1, 2), i(1), z(3, 2)
+
+
+def test_calls_without_derivatives_refuse_tensors_that_want_one():
+    from mlx_primitives.cache import paged_append, quantized_paged_attention
+    k, pool, bt, ctx, sc = _pool_args()
+    p8 = pool.to(torch.int8)
+    wants = lambda t: t.clone().requires_grad_(True)
+    for f in (lambda: paged_append(wants(k), k, pool, pool, bt, ctx), lambda: paged_append(k, wants(k), pool, pool, bt, ctx),
+              lambda: paged_append(k, k, wants(pool), pool, bt, ctx), lambda: paged_append(k, k, pool, wants(pool), bt, ctx),
+              lambda: paged_append(k, k, pool, pool, bt, ctx, q=wants(k)),
+              lambda: paged_append(k, k, pool, pool, bt, ctx, k_weight=wants(torch.ones(64))),
+              lambda: paged_append(k, k, p8, p8, bt, ctx, k_scales=wants(sc), v_scales=sc),
+              lambda: quantized_paged_attention(k, p8, p8, wants(sc), sc, bt, ctx),
+              lambda: quantized_paged_attention(k, p8, p8, sc, wants(sc), bt, ctx),
+              lambda: quantized_paged_attention(k, p8, p8, sc, sc, bt, ctx, alibi_slopes=wants(torch.ones(2)))):
+        with pytest.raises(NotImplementedError, match="differentiable"):
+            f()
+        with torch.no_grad():
+            try:
+                f()
+            except (ValueError, RuntimeError) as e:  # not that they want gradients
+                assert "CUDA" in str(e)

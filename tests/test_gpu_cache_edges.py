@@ -131,6 +131,32 @@ def test_attention_queries_near_the_largest_value(dtype, Sq):
     _check_attn(_attend(*case, scale=2.0 ** -36), *case, scale=2.0 ** -36)
 
 
+def test_gradients_that_would_be_lost_are_refused():
+    """Pools, scales and slopes that want gradients: no call drops them without a word."""
+    from mlx_primitives.cache import paged_append, quantized_paged_attention
+    rs = np.random.RandomState(46)
+    q, pools, scales, bt, ctx = _attn_case(rs, [100, 37], 4, 2, 64, 16, torch.float32, "e4m3")
+    bt, ctx = torch.from_numpy(bt).cuda(), torch.from_numpy(ctx).cuda()
+    wants = lambda t: t.clone().requires_grad_(True)
+    for args in ((*pools, wants(scales[0]), scales[1]), (*pools, scales[0], wants(scales[1]))):
+        with pytest.raises(NotImplementedError, match="differentiable"):
+            quantized_paged_attention(q, *args, bt, ctx)
+        with torch.no_grad():
+            assert torch.equal(quantized_paged_attention(q, *args, bt, ctx),
+                               quantized_paged_attention(q, *pools, *scales, bt, ctx))
+    with pytest.raises(NotImplementedError, match="differentiable"):
+        quantized_paged_attention(q, *pools, *scales, bt, ctx, alibi_slopes=wants(torch.ones(4, device="cuda")))
+    k = _rand(rs, (2, 1, 2, 64), torch.float32)
+    pool = torch.zeros(pools[0].shape, device="cuda")
+    with pytest.raises(NotImplementedError, match="differentiable"):
+        paged_append(k, k, wants(pool), pool.clone(), bt, ctx)
+    with pytest.raises(NotImplementedError, match="differentiable"):
+        paged_append(k, k, pool, wants(pool), bt, ctx)
+    with pytest.raises(NotImplementedError, match="differentiable"):
+        paged_append(k, k, *pools, bt, ctx, k_scales=wants(scales[0]), v_scales=scales[1])
+    assert not pool.any()
+
+
 def test_block_tables_shared_by_expansion():
     """One table for all sequences, as a view without a row stride."""
     from mlx_primitives.cache import paged_append, quantized_paged_attention
