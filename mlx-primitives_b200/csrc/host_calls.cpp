@@ -72,6 +72,8 @@ int cache_code_of(at::ScalarType s) {
 
 bool on(const Arg& a, int64_t dev) { return a->is_cuda() && a->get_device() == dev; }
 bool wants_grad(const Arg& a) { return a && a->requires_grad(); }
+// A forward-mode derivative, which no call here has.
+bool has_tangent(const Arg& a) { return a && a->_fw_grad(/*level=*/0).defined(); }
 
 // (batch, seq, heads, dim) tensor with unit dim stride.
 bool rows(const Arg& a, int64_t dev) { return a && a->dim() == 4 && on(a, dev) && a->stride(3) == 1; }
@@ -264,6 +266,8 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (qw && !(weight(qw, dev, D) && weight(kw, dev, D))) return none();
     if (c && !(table(c, dev, D / 2) && table(s, dev, D / 2) && c->size(0) == s->size(0))) return none();
     if (wants_grad(c) || wants_grad(s)) return none();
+    for (const Arg* x : {&q, &k, &qw, &kw, &c, &s})
+      if (has_tangent(*x)) return none();
     if (pos && (pos->scalar_type() != at::kInt || !on(pos, dev) || pos->dim() != 2 || pos->size(0) != B ||
                 pos->size(1) != q->size(1) || q->size(1) != k->size(1)))
       return none();
@@ -317,7 +321,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Arg k(a[0]), v(a[1]), kp(a[2]), vp(a[3]), bt(a[4]), ctx(a[5]), fresh(a[6]), q(a[7]), c(a[8]), s(a[9]),
         qw(a[10]), kw(a[11]), ks(a[12]), vs(a[13]);
     for (const Arg* x : {&k, &v, &kp, &vp, &bt, &ctx, &fresh, &q, &c, &s, &qw, &kw, &ks, &vs})
-      if (!x->ok) return none();
+      if (!x->ok || has_tangent(*x)) return none();
     if (!k || !v || !kp || !vp || !bt || !ctx || !k->is_cuda()) return none();
     const int64_t dev = k->get_device();
     const int code = code_of(k->scalar_type());
@@ -403,7 +407,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     const Arg q(a[0]), kp(a[1]), vp(a[2]), ks(a[3]), vs(a[4]), bt(a[5]), ctx(a[6]), lens(a[7]);
     for (const Arg* x : {&q, &kp, &vp, &ks, &vs, &bt, &ctx, &lens})
-      if (!x->ok) return none();
+      if (!x->ok || has_tangent(*x)) return none();
     if (!q || !kp || !vp || !bt || !ctx || !q->is_cuda()) return none();
     const int64_t dev = q->get_device();
     const int code = code_of(q->scalar_type());

@@ -15,6 +15,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 __all__ = [
     "MLXP_OK", "MLXP_ERR_INVALID", "MLXP_ERR_UNSUPPORTED", "MLXP_ERR_TIMEOUT",
@@ -180,6 +181,13 @@ def int32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     if t.dtype in _WIDE_INTS:
         t = t.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1)
     return t.to(device, torch.int32)
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """Raises where a tensor carries a forward-mode tangent, which `what` would drop."""
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def last_error() -> str:

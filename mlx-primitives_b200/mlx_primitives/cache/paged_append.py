@@ -140,6 +140,8 @@ def paged_append(
         raise ValueError(f"pools of (heads, head_dim) = {(Hp, Dp)} cannot take k of {(Hk, D)}")
     if D % 2 or D < 2:
         raise ValueError(f"head_dim must be even, got {D}")
+    _lib.refuse_tangents("paged_append", k, v, q, k_pool, v_pool, k_scales, v_scales, q_weight, k_weight,
+                         cos_cache, sin_cache)
     refuse_gradients("paged_append", k, v, q, k_pool, v_pool, k_scales, v_scales, q_weight, k_weight)
     dev = k.get_device()
     if dev < 0 or k_pool.get_device() != dev or v_pool.get_device() != dev or v.get_device() != dev:

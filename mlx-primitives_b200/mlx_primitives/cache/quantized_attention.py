@@ -99,6 +99,7 @@ def quantized_paged_attention(
         raise ValueError(f"alibi_slopes must be (num_heads,) = ({H},), got {tuple(alibi_slopes.shape)}")
     if window_size is not None and window_size < 0:
         raise ValueError(f"window_size must be >= 0, got {window_size}")
+    _lib.refuse_tangents("quantized_paged_attention", q, k_pool, v_pool, k_scales, v_scales, alibi_slopes)
     refuse_gradients("quantized_paged_attention", q, k_pool, v_pool, k_scales, v_scales, alibi_slopes)
     dev = q.get_device()
     host = dev < 0

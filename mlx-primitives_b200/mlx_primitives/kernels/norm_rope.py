@@ -186,6 +186,7 @@ def qk_norm_rope(
         return out
     if not _quick_ok(q, k, q_weight, k_weight, cos_cache, sin_cache, positions):
         _refuse(q, k, q_weight, k_weight, cos_cache, sin_cache, positions)
+    _lib.refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, cos_cache, sin_cache)
     needs = torch.is_grad_enabled() and (
         q.requires_grad or k.requires_grad
         or (q_weight is not None and (q_weight.requires_grad or k_weight.requires_grad)))

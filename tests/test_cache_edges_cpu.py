@@ -87,3 +87,23 @@ def test_calls_without_derivatives_refuse_tensors_that_want_one():
                 f()
             except (ValueError, RuntimeError) as e:  # not that they want gradients
                 assert "CUDA" in str(e)
+
+
+def test_tangents_are_refused_before_any_device_work():
+    import torch.autograd.forward_ad as fwd
+
+    from mlx_primitives.cache import paged_append, quantized_paged_attention
+    from mlx_primitives.kernels import qk_norm_rope
+    k, pool, bt, ctx, sc = _pool_args()
+    p8, w, cs = pool.to(torch.int8), torch.ones(64), torch.zeros(32, 32)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        for f in (lambda: qk_norm_rope(dual(k), k, w, w), lambda: qk_norm_rope(k, k, w, dual(w), cs, cs),
+                  lambda: qk_norm_rope(k, k, None, None, cs, dual(cs)),
+                  lambda: paged_append(k, dual(k), pool, pool, bt, ctx),
+                  lambda: paged_append(k, k, dual(pool), pool, bt, ctx),
+                  lambda: paged_append(k, k, pool, pool, bt, ctx, q=dual(k)),
+                  lambda: quantized_paged_attention(dual(k), p8, p8, sc, sc, bt, ctx),
+                  lambda: quantized_paged_attention(k, p8, p8, sc, dual(sc), bt, ctx)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()

@@ -131,6 +131,39 @@ def test_attention_queries_near_the_largest_value(dtype, Sq):
     _check_attn(_attend(*case, scale=2.0 ** -36), *case, scale=2.0 ** -36)
 
 
+def test_tangents_are_refused():
+    """Forward-mode derivatives are refused by the calls that take the short way, too."""
+    import torch.autograd.forward_ad as fwd
+
+    from mlx_primitives.cache import paged_append, quantized_paged_attention
+    from mlx_primitives.kernels import qk_norm_rope
+    rs = np.random.RandomState(43)
+    q, k, qw, kw = _norm_case(2, 7, 4, 2, 64, torch.float32)
+    qa, pools, scales, bt, ctx = _attn_case(rs, [100, 37], 4, 2, 64, 16, torch.float32, "e4m3")
+    bt, ctx = torch.from_numpy(bt).cuda(), torch.from_numpy(ctx).cuda()
+    cos, sin = _tables(16, 32)
+    before = [t.view(torch.uint8).clone() for t in pools]
+    with fwd.dual_level():
+        for grad in (False, True):
+            dual = lambda t: fwd.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))
+            for args in ((dual(q), k, qw, kw, cos, sin), (q, dual(k), qw, kw, cos, sin), (q, k, dual(qw), kw),
+                         (q, k, qw, kw, dual(cos), sin)):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    qk_norm_rope(*args)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                quantized_paged_attention(dual(qa), *pools, *scales, bt, ctx)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                quantized_paged_attention(qa, *pools, dual(scales[0]), scales[1], bt, ctx)
+            for which in range(2):
+                kv = [k[:, :1], k[:, 1:2]]
+                kv[which] = dual(kv[which])
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    paged_append(*kv, *pools, bt, ctx, k_scales=scales[0], v_scales=scales[1])
+        assert qk_norm_rope(q, k, qw, kw)[0].shape == q.shape  # without tangents: as ever
+    for a, b in zip(pools, before):
+        assert torch.equal(a.view(torch.uint8), b)
+
+
 def test_gradients_that_would_be_lost_are_refused():
     """Pools, scales and slopes that want gradients: no call drops them without a word."""
     from mlx_primitives.cache import paged_append, quantized_paged_attention
