@@ -15,6 +15,7 @@
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -121,15 +122,13 @@ bool scales(const Arg& k, const Arg& v, int64_t dev, int64_t blocks, int64_t hea
   return true;
 }
 
-// Every function: C++ exceptions become Python's.
+// Every function: C++ exceptions become Python's, as torch's own calls have them (running out of
+// memory among them, which callers catch by its type).
 template <typename F>
 PyObject* guarded(F&& f) {
-  try {
-    return f();
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  HANDLE_TH_ERRORS
+  return f();
+  END_HANDLE_TH_ERRORS
 }
 
 // ---- norm + rotation, with its gradient -------------------------------------------------------

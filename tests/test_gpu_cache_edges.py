@@ -164,6 +164,29 @@ def test_tangents_are_refused():
         assert torch.equal(a.view(torch.uint8), b)
 
 
+def test_running_out_of_memory_keeps_its_type():
+    """The allocator's own exception, which callers catch to go on with less, by the short way as by
+    the long one."""
+    from mlx_primitives.cache import paged_append, quantized_paged_attention
+    from mlx_primitives.kernels import qk_norm_rope
+    w = torch.ones(64, device="cuda")
+    wide = torch.ones(1, 1, 1, 64, dtype=torch.bfloat16, device="cuda").expand(1 << 20, 1, 32, 64)  # 4 GB once dense
+    pool = torch.zeros(2, 16, 32, 64, dtype=torch.bfloat16, device="cuda")
+    p8, sc = pool.to(torch.float8_e4m3fn), torch.ones(2, 32, device="cuda")
+    bt = torch.zeros(1 << 20, 1, dtype=torch.int32, device="cuda")
+    none = torch.zeros(1 << 20, dtype=torch.int32, device="cuda")
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.01)
+    try:
+        for f in (lambda: qk_norm_rope(wide, wide, w, w),
+                  lambda: paged_append(wide, wide, pool, pool.clone(), bt, none, new_lens=none, q=wide),
+                  lambda: quantized_paged_attention(wide, p8, p8.clone(), sc, sc, bt, none)):
+            with pytest.raises(torch.OutOfMemoryError):
+                f()
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+
+
 def test_gradients_that_would_be_lost_are_refused():
     """Pools, scales and slopes that want gradients: no call drops them without a word."""
     from mlx_primitives.cache import paged_append, quantized_paged_attention
