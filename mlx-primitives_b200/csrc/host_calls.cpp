@@ -131,6 +131,13 @@ PyObject* guarded(F&& f) {
   END_HANDLE_TH_ERRORS
 }
 
+// The interpreter is free to run other threads while this lives: around allocations and launches,
+// which wait where the allocator or the launch queue is full.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 // ---- norm + rotation, with its gradient -------------------------------------------------------
 
 // What the forward and the backward have in common; undefined tensors are not there.
@@ -278,15 +285,18 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const bool graph =
         at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(qw) || wants_grad(kw));
     at::Tensor qo, ko;
+    int rc;
     {
+      const Unlocked others;
       at::AutoDispatchBelowADInplaceOrView below;  // plain allocations
       qo = rows_like(*q.t);
       ko = rows_like(*k.t);
+      auto x = norm_rope_args(*q.t, *k.t, or_none(qw), or_none(kw), or_none(c), or_none(s), or_none(pos), offset,
+                              k_offset, eps);
+      set_outputs(x, qo, ko);
+      rc = g_norm_rope(&x);
     }
-    auto x = norm_rope_args(*q.t, *k.t, or_none(qw), or_none(kw), or_none(c), or_none(s), or_none(pos), offset,
-                            k_offset, eps);
-    set_outputs(x, qo, ko);
-    if (const int rc = g_norm_rope(&x)) return PyLong_FromLong(rc);
+    if (rc) return PyLong_FromLong(rc);
     if (graph) {
       auto node = std::shared_ptr<NormRopeBackward>(new NormRopeBackward(), torch::autograd::deleteNode);
       node->set_next_edges(torch::autograd::collect_next_edges(*q.t, *k.t, or_none(qw), or_none(kw)));
@@ -351,14 +361,10 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (wants_grad(*x)) return none();
     mlxp_paged_append_args x{};
     x.size = sizeof(x);
-    at::Tensor qo;
     if (q) {
-      qo = rows_like(*q.t);
       x.q = q.data();
-      x.q_out = qo.data_ptr();
       x.Hq = q->size(2);
       seq_strides(x.q_strides, *q.t);
-      seq_strides(x.q_out_strides, qo);
     }
     x.k = k.data();
     x.v = v.data();
@@ -393,7 +399,18 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       for (int i = 0; i < 2; ++i) x.scale_strides[i] = ks->stride(i);
     x.eps = PyFloat_AS_DOUBLE(a[14]);
     x.stream = stream_of(dev);
-    if (const int rc = g_append(&x)) return PyLong_FromLong(rc);
+    at::Tensor qo;
+    int rc;
+    {
+      const Unlocked others;
+      if (q) {
+        qo = rows_like(*q.t);
+        x.q_out = qo.data_ptr();
+        seq_strides(x.q_out_strides, qo);
+      }
+      rc = g_append(&x);
+    }
+    if (rc) return PyLong_FromLong(rc);
     if (!q) Py_RETURN_TRUE;
     return THPVariable_Wrap(std::move(qo));
   });
@@ -424,11 +441,9 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (at::GradMode::is_enabled())
       for (const Arg* x : {&q, &kp, &vp, &ks, &vs})
         if (wants_grad(*x)) return none();
-    at::Tensor o = at::empty_like(*q.t);
     mlxp_quant_paged_attn_args x{};
     x.size = sizeof(x);
     x.q = q.data();
-    x.o = o.data_ptr();
     x.k_pool = kp.data();
     x.v_pool = vp.data();
     x.k_scales = static_cast<const float*>(ks.data());
@@ -451,15 +466,23 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     x.window = PyLong_AsLongLong(a[10]);
     if (PyErr_Occurred()) return nullptr;
     seq_strides(x.q_strides, *q.t);
-    seq_strides(x.o_strides, o);
     for (int i = 0; i < 3; ++i) x.pool_strides[i] = kp->stride(i);
     for (int i = 0; i < 2; ++i) x.scale_strides[i] = ks->stride(i);
     x.scale = a[8] == Py_None ? 1.0 / std::sqrt((double)D) : PyFloat_AS_DOUBLE(a[8]);
     x.stream = stream_of(dev);
-    x.ws_bytes = g_attn_ws(&x);
-    at::Tensor ws = at::empty({(int64_t)x.ws_bytes}, q->options().dtype(at::kByte));
-    x.workspace = ws.data_ptr();
-    if (const int rc = g_attn(&x)) return PyLong_FromLong(rc);
+    at::Tensor o;
+    int rc;
+    {
+      const Unlocked others;
+      o = at::empty_like(*q.t);
+      x.o = o.data_ptr();
+      seq_strides(x.o_strides, o);
+      x.ws_bytes = g_attn_ws(&x);
+      const at::Tensor ws = at::empty({(int64_t)x.ws_bytes}, q->options().dtype(at::kByte));
+      x.workspace = ws.data_ptr();
+      rc = g_attn(&x);
+    }
+    if (rc) return PyLong_FromLong(rc);
     return THPVariable_Wrap(std::move(o));
   });
 }

@@ -2,7 +2,11 @@
 their scales, masks and sizes, autograd's other modes, and the ways a call can take to the kernels.
 Tolerances are those of that file, which derives them."""
 
+import ctypes
 import math
+import subprocess
+import threading
+import time
 
 import numpy as np
 import pytest
@@ -185,6 +189,50 @@ def test_running_out_of_memory_keeps_its_type():
                 f()
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
+
+
+def test_launches_let_other_threads_run(tmp_path):
+    """While a call sits in the library (a full launch queue), other Python threads go on.  The
+    library's functions are replaced by one that sleeps and returns a status."""
+    from mlx_primitives import _lib
+    from mlx_primitives.cache import paged_append, quantized_paged_attention
+    from mlx_primitives.kernels import qk_norm_rope
+    src = tmp_path / "slow.c"
+    src.write_text("#include <unistd.h>\nint slow(const void* a) { (void)a; usleep(400000); return 1; }\n")
+    so = tmp_path / "slow.so"
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(so), str(src)], check=True)
+    address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
+    slow, L = address(ctypes.CDLL(str(so)).slow), _lib.lib()
+    rs = np.random.RandomState(44)
+    q, k, w, _ = _norm_case(2, 1, 4, 2, 64, torch.float32)
+    qa, pools, scales, bt, ctx = _attn_case(rs, [100, 37], 4, 2, 64, 16, torch.float32, "e4m3")
+    bt, ctx = torch.from_numpy(bt).cuda(), torch.from_numpy(ctx).cuda()
+    host = _lib.calls()
+    host.bind(slow, address(L.mlxp_qk_norm_rope_bwd), address(L.mlxp_qk_norm_rope_bwd_workspace_size), slow, slow,
+              address(L.mlxp_quant_paged_attn_workspace_size))
+    try:
+        for f in (lambda: qk_norm_rope(q, k, w, w),
+                  lambda: paged_append(k, k, *pools, bt, ctx, k_scales=scales[0], v_scales=scales[1]),
+                  lambda: quantized_paged_attention(qa, *pools, *scales, bt, ctx)):
+            failed = []
+
+            def work():
+                try:
+                    f()
+                except ValueError as e:  # status 1
+                    failed.append(e)
+            t = threading.Thread(target=work)
+            t.start()
+            turns = 0
+            while t.is_alive():
+                time.sleep(0.01)
+                turns += 1
+            t.join()
+            assert failed and turns >= 10, turns
+    finally:
+        _lib._calls = None
+        _lib.calls()
+    assert qk_norm_rope(q, k, w, w)[0].shape == q.shape
 
 
 def test_gradients_that_would_be_lost_are_refused():
