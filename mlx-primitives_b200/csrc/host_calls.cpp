@@ -21,6 +21,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <cmath>
 #include <memory>
@@ -411,6 +412,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       rc = g_append(&x);
     }
     if (rc) return PyLong_FromLong(rc);
+    for (const Arg* t : {&kp, &vp, &ks, &vs})  // written in place: saved copies are stale
+      if (*t && !(*t)->is_inference()) torch::autograd::impl::bump_version(*t->t);
     if (!q) Py_RETURN_TRUE;
     return THPVariable_Wrap(std::move(qo));
   });

@@ -222,6 +222,7 @@ def paged_append(
             ps[0], ps[1], ps[2], sc[0], sc[1], eps, _lib.raw_stream(dev)))
     if rc:
         _lib.check(rc, "mlxp_paged_append")
+    torch.autograd.graph.increment_version((k_pool, v_pool, k_scales, v_scales) if quant else (k_pool, v_pool))
     return q_out
 
 

@@ -14,7 +14,7 @@ import torch
 
 from oracle import cache_oracle as C
 from test_gpu_cache_ops import (TYPES, _attend, _attn_case, _check_attn, _check_norm, _close, _n, _norm_case,
-                                _rand, _tables)
+                                _pool_case, _rand, _tables)
 
 pytestmark = pytest.mark.gpu
 
@@ -233,6 +233,36 @@ def test_launches_let_other_threads_run(tmp_path):
         _lib._calls = None
         _lib.calls()
     assert qk_norm_rope(q, k, w, w)[0].shape == q.shape
+
+
+@pytest.mark.parametrize("ints", [torch.int32, torch.int64])
+@pytest.mark.parametrize("kind", [None, "e4m3"])
+def test_append_marks_the_pools_as_changed(ints, kind):
+    """Autograd sees that the pools (and scales) were written: a gradient that needs their old
+    values is refused.  Inference tensors, which have no such mark, are written all the same."""
+    from mlx_primitives.cache import paged_append
+    rs = np.random.RandomState(45)
+    bt, pools, scales = _pool_case(rs, [20, 30], 16, 2, 64, torch.float32, kind)
+    k = _rand(rs, (2, 3, 2, 64), torch.float32)
+    bt, ctx = torch.from_numpy(bt).cuda().to(ints), torch.tensor([5, 16], device="cuda").to(ints)
+
+    def call(p, s):
+        paged_append(k, k, *p, bt, ctx, k_scales=s[0], v_scales=s[1])
+    for t in [*pools, *scales][:2 if kind is None else 4]:
+        w = torch.ones_like(t, dtype=torch.float32).requires_grad_(True)
+        read = t if t.dtype is torch.float32 else t.view(torch.uint8)
+        y = (w * read).sum() if t.dtype is torch.float32 else None
+        was = t._version
+        call(pools, scales)
+        assert t._version > was
+        if y is not None:
+            with pytest.raises(RuntimeError, match="inplace"):
+                y.backward()
+    with torch.inference_mode():
+        frozen = [t.clone() for t in pools]
+        fs = [None if s is None else s.clone() for s in scales]
+    call(frozen, fs)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(frozen, pools))
 
 
 def test_gradients_that_would_be_lost_are_refused():
