@@ -13,6 +13,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -22,12 +23,14 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/dynamo/compiled_autograd.h>
 
 #include <cmath>
 #include <memory>
 #include <mutex>
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 #include "../../include/mlxp_attn.h"
 
@@ -194,10 +197,64 @@ void set_outputs(mlxp_qk_norm_rope_args& x, const at::Tensor& qo, const at::Tens
 
 using torch::autograd::variable_list;
 
+// What the gradient needs, once unpacked.
+struct NormRopeSaved {
+  at::Tensor t[7];  // q, k, their weights, cos, sin, positions; the last five may be undefined
+  int64_t offset = 0, k_offset = 0;
+  double eps = 0;
+};
+
+// Gradients of q, k and the weights from those of the outputs, either of which may be undefined.
+variable_list norm_rope_gradients(const NormRopeSaved& a, variable_list g, bool want_qw, bool want_kw) {
+  const at::Tensor &q = a.t[0], &k = a.t[1], &qw = a.t[2], &kw = a.t[3];
+  for (at::Tensor& t : g)
+    if (t.defined() && t.stride(3) != 1) t = t.contiguous();
+  variable_list out(4);
+  const c10::OptionalDeviceGuard device(q.device());
+  at::AutoDispatchBelowADInplaceOrView below;  // plain allocations
+  if (g[0].defined()) out[0] = rows_like(q);
+  if (g[1].defined()) out[1] = rows_like(k);
+  if (qw.defined() && want_qw) out[2] = at::empty_like(qw);
+  if (kw.defined() && want_kw) out[3] = at::empty_like(kw);
+  auto x = norm_rope_args(q, k, qw, kw, a.t[4], a.t[5], a.t[6], a.offset, a.k_offset, a.eps);
+  set_outputs(x, out[0], out[1]);
+  if (g[0].defined()) {
+    x.gq = g[0].data_ptr();
+    seq_strides(x.gq_strides, g[0]);
+  }
+  if (g[1].defined()) {
+    x.gk = g[1].data_ptr();
+    seq_strides(x.gk_strides, g[1]);
+  }
+  at::Tensor ws;
+  if (out[2].defined() || out[3].defined()) {
+    if (out[2].defined()) x.dq_weight = out[2].data_ptr();
+    if (out[3].defined()) x.dk_weight = out[3].data_ptr();
+    x.ws_bytes = g_norm_rope_ws(x.D);
+    ws = at::empty({(int64_t)x.ws_bytes}, q.options().dtype(at::kByte));
+    x.workspace = ws.data_ptr();
+  }
+  if (const int rc = g_norm_rope_bwd(&x))
+    throw std::runtime_error("mlxp_qk_norm_rope_bwd failed with status " + std::to_string(rc));
+  return out;
+}
+
+// The same as a captured backward (compiled autograd) calls it, its arguments packed below.
+variable_list norm_rope_gradients_packed(const variable_list& g, const std::vector<c10::IValue>& args) {
+  torch::dynamo::autograd::PackedArgs p(args);
+  NormRopeSaved a;
+  for (at::Tensor& t : a.t) t = p.unpack<at::Tensor>();
+  a.offset = p.unpack<int64_t>();
+  a.k_offset = p.unpack<int64_t>();
+  a.eps = p.unpack<double>();
+  const bool want_qw = p.unpack<bool>(), want_kw = p.unpack<bool>();
+  return norm_rope_gradients(a, g, want_qw, want_kw);
+}
+
 // The graph's node.  A Node of its own rather than torch::autograd::Function: that one's context
 // and wrapping of outputs cost as much as the launches.
 struct NormRopeBackward : torch::autograd::Node {
-  torch::autograd::SavedVariable q_, k_, qw_, kw_, c_, s_, pos_;
+  torch::autograd::SavedVariable saved_[7];  // in NormRopeSaved's order
   int64_t offset = 0, k_offset = 0;
   double eps = 0;
 
@@ -205,43 +262,22 @@ struct NormRopeBackward : torch::autograd::Node {
 
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    for (auto* v : {&q_, &k_, &qw_, &kw_, &c_, &s_, &pos_}) v->reset_data();
+    for (auto& v : saved_) v.reset_data();
+  }
+
+  NormRopeSaved unpack() const {
+    NormRopeSaved a;
+    for (int i = 0; i < 7; ++i) a.t[i] = saved_[i].unpack();
+    a.offset = offset;
+    a.k_offset = k_offset;
+    a.eps = eps;
+    return a;
   }
 
   variable_list apply(variable_list&& g) override {
     std::lock_guard<std::mutex> lock(mutex_);
-    const at::Tensor q = q_.unpack(), k = k_.unpack(), qw = qw_.unpack(), kw = kw_.unpack(), c = c_.unpack(),
-                     s = s_.unpack(), pos = pos_.unpack();
-    for (at::Tensor& t : g)
-      if (t.defined() && t.stride(3) != 1) t = t.contiguous();
-    variable_list out(4);
-    {
-      at::AutoDispatchBelowADInplaceOrView below;  // plain allocations
-      if (g[0].defined()) out[0] = rows_like(q);
-      if (g[1].defined()) out[1] = rows_like(k);
-      if (qw.defined() && task_should_compute_output(2)) out[2] = at::empty_like(qw);
-      if (kw.defined() && task_should_compute_output(3)) out[3] = at::empty_like(kw);
-      auto x = norm_rope_args(q, k, qw, kw, c, s, pos, offset, k_offset, eps);
-      set_outputs(x, out[0], out[1]);
-      if (g[0].defined()) {
-        x.gq = g[0].data_ptr();
-        seq_strides(x.gq_strides, g[0]);
-      }
-      if (g[1].defined()) {
-        x.gk = g[1].data_ptr();
-        seq_strides(x.gk_strides, g[1]);
-      }
-      at::Tensor ws;
-      if (out[2].defined() || out[3].defined()) {
-        if (out[2].defined()) x.dq_weight = out[2].data_ptr();
-        if (out[3].defined()) x.dk_weight = out[3].data_ptr();
-        x.ws_bytes = g_norm_rope_ws(x.D);
-        ws = at::empty({(int64_t)x.ws_bytes}, q.options().dtype(at::kByte));
-        x.workspace = ws.data_ptr();
-      }
-      if (const int rc = g_norm_rope_bwd(&x))
-        throw std::runtime_error("mlxp_qk_norm_rope_bwd failed with status " + std::to_string(rc));
-    }
+    variable_list out =
+        norm_rope_gradients(unpack(), std::move(g), task_should_compute_output(2), task_should_compute_output(3));
     if (at::GradMode::is_enabled()) {  // gradients of these are refused when they are asked for
       variable_list there;
       for (const at::Tensor& t : out)
@@ -253,6 +289,42 @@ struct NormRopeBackward : torch::autograd::Node {
       for (at::Tensor& t : out)
         if (t.defined()) t = there[i++];
     }
+    return out;
+  }
+
+  // Compiled autograd: what tells two nodes apart, and the node as one opaque call of the capture.
+  void compiled_args(torch::dynamo::autograd::CompiledNodeArgs& args) const override {
+    for (const auto& v : saved_) args.collect(v, /*is_output=*/false);
+    args.collect(offset);
+    args.collect(k_offset);
+    args.collect(eps);
+  }
+
+  variable_list apply_with_saved(const variable_list& g, torch::dynamo::autograd::SwapSavedVariables& swap) override {
+    namespace ca = torch::dynamo::autograd;
+    for (auto& v : saved_) swap.before(v);
+    const NormRopeSaved a = unpack();
+    ca::PackedArgs p;
+    std::vector<at::TypePtr> schema;
+    for (const at::Tensor& t : a.t) {
+      p.pack(t);
+      schema.push_back(at::TensorType::get());
+    }
+    p.pack(a.offset);
+    p.pack(a.k_offset);
+    p.pack(a.eps);
+    p.pack(task_should_compute_output(2));
+    p.pack(task_should_compute_output(3));
+    schema.insert(schema.end(), {at::IntType::get(), at::IntType::get(), at::FloatType::get(), at::BoolType::get(),
+                                 at::BoolType::get()});
+    const auto& compiler = ca::getPyCompilerInterface();
+    const std::string fn = compiler->bind_function(swap.get_py_compiler(), name(), norm_rope_gradients_packed, schema,
+                                                   /*is_custom_function=*/true, /*is_traceable=*/false);
+    variable_list out = compiler->call_function(
+        swap.get_py_compiler(), "apply_functional", fn, g, std::move(p).vec(),
+        ca::IValuePacker<std::vector<std::optional<torch::autograd::InputMetadata>>>::pack(
+            ca::get_input_metadata(next_edges())));
+    for (auto& v : saved_) swap.after(v);
     return out;
   }
 };
@@ -301,14 +373,8 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (graph) {
       auto node = std::shared_ptr<NormRopeBackward>(new NormRopeBackward(), torch::autograd::deleteNode);
       node->set_next_edges(torch::autograd::collect_next_edges(*q.t, *k.t, or_none(qw), or_none(kw)));
-      using torch::autograd::SavedVariable;
-      node->q_ = SavedVariable(*q.t, false);
-      node->k_ = SavedVariable(*k.t, false);
-      node->qw_ = SavedVariable(or_none(qw), false);
-      node->kw_ = SavedVariable(or_none(kw), false);
-      node->c_ = SavedVariable(or_none(c), false);
-      node->s_ = SavedVariable(or_none(s), false);
-      node->pos_ = SavedVariable(or_none(pos), false);
+      const at::Tensor* keep[7] = {q.t, k.t, &or_none(qw), &or_none(kw), &or_none(c), &or_none(s), &or_none(pos)};
+      for (int i = 0; i < 7; ++i) node->saved_[i] = torch::autograd::SavedVariable(*keep[i], /*is_output=*/false);
       node->offset = offset;
       node->k_offset = k_offset;
       node->eps = eps;

@@ -345,3 +345,30 @@ def test_integers_past_32_bits():
                  new_lens=torch.tensor([far, -far]).cuda(), k_scales=scales[0], v_scales=scales[1])
     same = [torch.equal(p.view(torch.uint8)[bt[b, 0]], w[bt[b, 0]]) for p, w in zip(pools, before) for b in range(2)]
     assert same == [False, True, False, True]
+
+
+def test_norm_rope_under_compiled_autograd():
+    """The graph's node is one that a captured backward takes, as a call of its own."""
+    from torch._dynamo import compiled_autograd
+
+    from mlx_primitives.kernels import qk_norm_rope
+    q, k, qw, kw = _norm_case(2, 9, 4, 2, 64, torch.float32)
+    cos, sin = _tables(16, 32)
+    pos = torch.tensor([[0, 1, 2, 3, 4, 5, 6, -1, -1], [3, 4, 5, 6, 7, 8, 9, 10, 11]], dtype=torch.int32, device="cuda")
+
+    def grads(leaves, how, **kw_):
+        leaves = [t.clone().requires_grad_(want) for t, want in leaves]
+        out = qk_norm_rope(*leaves, **kw_)
+        y = out[0].sin().sum() + (out[1] * 2).sum()
+        with how():
+            y.backward()
+        return [t.grad for t in leaves]
+    import contextlib
+    for wants in ((True,) * 4, (True, False, False, True), (False, False, True, False)):
+        for kw_ in (dict(cos_cache=cos, sin_cache=sin), dict(cos_cache=cos, sin_cache=sin, positions=pos),
+                    dict(eps=1e-3), dict(cos_cache=cos, sin_cache=sin, offset=2, k_offset=5)):
+            leaves = list(zip((q, k, qw, kw), wants))
+            want = grads(leaves, contextlib.nullcontext, **kw_)
+            got = grads(leaves, lambda: compiled_autograd._enable(lambda gm: gm), **kw_)
+            for a, b in zip(got, want):
+                assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
