@@ -13,8 +13,8 @@ import pytest
 import torch
 
 from oracle import cache_oracle as C
-from test_gpu_cache_ops import (TYPES, _attend, _attn_case, _check_attn, _check_norm, _close, _n, _norm_case,
-                                _pool_case, _rand, _tables)
+from test_gpu_cache_ops import (TYPES, _amp, _attend, _attn_case, _check_append, _check_attn, _check_norm,
+                                _close, _n, _norm_case, _pool_case, _rand, _tables)
 
 pytestmark = pytest.mark.gpu
 
@@ -372,3 +372,168 @@ def test_norm_rope_under_compiled_autograd():
             got = grads(leaves, lambda: compiled_autograd._enable(lambda gm: gm), **kw_)
             for a, b in zip(got, want):
                 assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+
+
+class _Spy:
+    """The short calls, with a record of whether each was taken."""
+
+    def __init__(self, real):
+        self.real, self.taken = real, []
+
+    def __getattr__(self, name):
+        def call(*args):
+            out = getattr(self.real, name)(*args)
+            self.taken.append(out is not None)
+            return out
+        return call
+
+
+@pytest.fixture
+def spy(monkeypatch):
+    from mlx_primitives import _lib
+    s = _Spy(_lib.calls())
+    monkeypatch.setattr(_lib, "calls", lambda: s)
+    return s
+
+
+@pytest.mark.parametrize("ints", [torch.int32, torch.int64])
+@pytest.mark.parametrize("dtype,D,kind,block", [("bf16", 128, None, 16), ("fp16", 64, None, 24), ("fp32", 64, "int8", 128),
+                                                ("bf16", 128, "e4m3", 16), ("bf16", 10, "int8", 5)])
+def test_append_by_either_way(spy, ints, dtype, D, kind, block):
+    """Everything that an append takes, by the short way (32-bit integers) and by the long one."""
+    from mlx_primitives.cache import paged_append
+    rs = np.random.RandomState(D + block)
+    dt, Hk, Hq, S = TYPES[dtype], 3, 5, 19
+    ctx = np.array([0, 1, 33, block, 4 * block - 1])
+    new = np.array([S, S - 3, 0, S, 1])
+    bt, pools, scales = _pool_case(rs, ctx + new, block, Hk, D, dt, kind)
+    k, v = (_rand(rs, (5, S, Hk, D), dt, 2.0) for _ in range(2))
+    fused = _rand(rs, (5, S, Hq + 2, D), dt, 2.0)
+    v = v.transpose(1, 2).contiguous().transpose(1, 2)  # strides of their own for each of k, v, q
+    q = fused[:, :, 1:Hq + 1]
+    cos, sin = _tables(bt.shape[1] * block, D // 2)
+    qw, kw = (1 + 0.1 * _rand(rs, (D,), torch.float32)).bfloat16(), 1 + 0.1 * _rand(rs, (D,), torch.float32)
+    at = np.where(np.arange(S) < new[:, None], ctx[:, None] + np.arange(S), -1)
+    before = [_n(t) if t is not None else None for t in (*pools, *scales)]
+    qo = paged_append(k, v, *pools, torch.from_numpy(bt).cuda().to(ints), torch.from_numpy(ctx).cuda().to(ints),
+                      new_lens=torch.from_numpy(new).cuda().to(ints), q=q, cos_cache=cos, sin_cache=sin, q_weight=qw,
+                      k_weight=kw, eps=1e-3, k_scales=scales[0], v_scales=scales[1])
+    assert spy.taken == [ints is torch.int32]
+    k64 = C.norm_rope(_n(k), _n(kw), _n(cos), _n(sin), at, 1e-3)
+    _check_append(k64, _n(v), True, before, pools, scales, bt, ctx, new, kind, dt)
+    want = C.norm_rope(_n(q), _n(qw), _n(cos), _n(sin), at, 1e-3)
+    _close(qo, want, dt, 2.0 ** -19 * _amp(want))
+
+
+@pytest.mark.parametrize("ints", [torch.int32, torch.int64])
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("fp32", 64), ("fp16", 6)])
+def test_norm_rope_by_either_way(spy, ints, dtype, D):
+    """Positions (strided ones) with padding, and the gradients, by the short way and by the long."""
+    from mlx_primitives.kernels import qk_norm_rope
+    leaves = [t.requires_grad_(True) for t in _norm_case(3, 20, 5, 2, D, TYPES[dtype], seed=D)]
+    cos, sin = _tables(40, D // 2)
+    pos = np.random.RandomState(D).randint(0, 40, (3, 20))
+    pos[0, 11:], pos[2, :4] = -1, -1
+    wide = torch.zeros(20, 6, dtype=ints, device="cuda")
+    wide[:, ::2] = torch.from_numpy(pos.T).cuda().to(ints)
+    out = qk_norm_rope(*leaves, cos, sin, positions=wide[:, ::2].T, eps=1e-3)
+    assert spy.taken == [ints is torch.int32]
+    _check_norm(*leaves, cos, sin, pos, out, 1e-3)
+    _check_gradients(leaves, out, pos, cos, sin, 1e-3, 6)
+    out = qk_norm_rope(*[t.detach() for t in leaves], cos, sin, offset=7, k_offset=20)
+    assert spy.taken[1]
+    for x, w, y, off in ((leaves[0], leaves[2], out[0], 7), (leaves[1], leaves[3], out[1], 20)):
+        want = C.norm_rope(_n(x), _n(w), _n(cos), _n(sin), np.tile(off + np.arange(20), (3, 1)))
+        _close(y, want, x.dtype, 2.0 ** -20 * 2 * _amp(want))
+
+
+@pytest.mark.parametrize("ints", [torch.int32, torch.int64])
+@pytest.mark.parametrize("Sq", [1, 70])
+def test_attention_by_either_way(spy, ints, Sq):
+    from mlx_primitives.cache import quantized_paged_attention
+    rs = np.random.RandomState(49)
+    q, pools, scales, bt, ctx = _attn_case(rs, [Sq + 90, 300, 33], 4, 2, 64, 16, torch.bfloat16, "e4m3", Sq=Sq)
+    q = q.transpose(1, 2).contiguous().transpose(1, 2)
+    ql = np.array([Sq, 0, min(Sq, 33)], dtype=np.int32)
+    t = lambda a: torch.from_numpy(a).cuda().to(ints)
+    out = quantized_paged_attention(q, *pools, *scales, t(bt), t(ctx), 0.25, True, 80, t(ql))
+    assert spy.taken == [ints is torch.int32]
+    _check_attn(out, q, pools, scales, bt, ctx, scale=0.25, window_size=80, query_lens=ql)
+
+
+def _sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+@pytest.mark.parametrize("dtype,D,Hq,Hk", [("bf16", 64, 19, 9), ("fp32", 64, 19, 2), ("fp16", 10, 3, 1),
+                                           ("bf16", 128, 33, 5)])
+def test_norm_rope_with_tokens_for_every_warp(spy, dtype, D, Hq, Hk):
+    """From 24 tokens an SM a warp takes all heads of a token, some rows at a time."""
+    from mlx_primitives.kernels import qk_norm_rope
+    B, S = 2, 13 * _sms() + 1
+    leaves = [t.requires_grad_(True) for t in _norm_case(B, S, Hq, Hk, D, TYPES[dtype], seed=D)]
+    cos, sin = _tables(S, D // 2)
+    pos = np.tile(np.arange(S), (B, 1))
+    pos[1, S // 2:] = -1
+    with torch.no_grad():
+        leaves[0][1, S // 2:] = float("nan")
+    out = qk_norm_rope(*leaves, cos, sin, positions=torch.from_numpy(pos).int().cuda())
+    assert spy.taken == [True]
+    _check_norm(*leaves, cos, sin, pos, out)
+    _check_gradients(leaves, out, pos, cos, sin, 1e-6, 7)
+
+
+@pytest.mark.parametrize("kind", [None, "e4m3", "int8"])
+def test_append_of_long_prompts(spy, kind):
+    """From 64 query rows' units an SM the queries take a launch of their own beside an 8-bit pool;
+    ragged prompts, some of them longer than others by orders."""
+    from mlx_primitives.cache import paged_append
+    rs = np.random.RandomState(50)
+    B, S, Hq, Hk, D, block, dt = 3, 22 * _sms(), 19, 2, 64, 16, torch.bfloat16
+    ctx, new = np.array([100, 0, 7]), np.array([S, 5, S - 1001])
+    bt, pools, scales = _pool_case(rs, ctx + new, block, Hk, D, dt, kind)
+    q, k, v = (_rand(rs, (B, S, h, D), dt, 2.0) for h in (Hq, Hk, Hk))
+    cos, sin = _tables(bt.shape[1] * block, D // 2)
+    qw, kw = (1 + 0.1 * _rand(rs, (D,), torch.float32) for _ in range(2))
+    at = np.where(np.arange(S) < new[:, None], ctx[:, None] + np.arange(S), -1)
+    before = [_n(t) if t is not None else None for t in (*pools, *scales)]
+    ints = lambda a: torch.from_numpy(a).int().cuda()
+    qo = paged_append(k, v, *pools, ints(bt), ints(ctx), new_lens=ints(new), q=q, cos_cache=cos, sin_cache=sin,
+                      q_weight=qw, k_weight=kw, k_scales=scales[0], v_scales=scales[1])
+    assert spy.taken == [True]
+    k64 = C.norm_rope(_n(k), _n(kw), _n(cos), _n(sin), at)
+    _check_append(k64, _n(v), True, before, pools, scales, bt, ctx, new, kind, dt)
+    want = C.norm_rope(_n(q), _n(qw), _n(cos), _n(sin), at)
+    _close(qo, want, dt, 2.0 ** -19 * _amp(want))
+
+
+@pytest.mark.parametrize("block,kw", [(8, dict()), (24, dict()), (16, dict(alibi=True)), (48, dict(alibi=True)),
+                                      (20, dict(window_size=60))])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_attention_of_chunks_outside_the_many_row_kernel(block, kw, dtype):
+    """64 rows a pool head and more with blocks that are not multiples of 16, ALiBi, or in fp32."""
+    from mlx_primitives.cache import get_alibi_slopes
+    rs = np.random.RandomState(51)
+    case = _attn_case(rs, [300, 90, 1000], 8, 2, 64, block, TYPES[dtype], "e4m3", Sq=70)
+    kw = {"alibi_slopes": get_alibi_slopes(8).numpy()} if kw.get("alibi") else kw
+    _check_attn(_attend(*case, **kw), *case, **kw)
+
+
+@pytest.mark.parametrize("block", [64, 24])
+def test_attention_past_32_bits(block):
+    """Blocks behind the first 2^31 elements of a pool, in each kernel."""
+    rs = np.random.RandomState(52)
+    Hk, D = 8, 128
+    nblk = (1 << 31) // (block * Hk * D) + 40
+    pools = [torch.zeros(nblk, block, Hk, D, dtype=torch.int8, device="cuda") for _ in range(2)]
+    n = np.array([500, 77], dtype=np.int32)
+    bt = (nblk - 1 - rs.permutation(2 * 21).reshape(2, 21)).astype(np.int32)
+    near = nblk - 42  # the oracle's pools hold the last blocks alone
+    scales = [torch.ones(nblk, Hk, device="cuda") for _ in range(2)]
+    for p, s in zip(pools, scales):
+        p[near:] = torch.randint(-127, 128, (42, block, Hk, D), device="cuda", dtype=torch.int8)
+        s[near:] = 2.0 ** -6 * (1 + torch.rand(42, Hk, device="cuda"))
+    for Sq in (1, 70):
+        q = _rand(rs, (2, Sq, 8, D), torch.bfloat16)
+        out = _attend(q, pools, scales, bt, n)
+        _check_attn(out, q, [p[near:] for p in pools], [s[near:] for s in scales], bt - near, n)
