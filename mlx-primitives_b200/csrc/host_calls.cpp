@@ -47,6 +47,7 @@ size_t (*g_attn_ws)(const mlxp_quant_paged_attn_args*) = nullptr;
 struct Arg {
   const at::Tensor* t = nullptr;
   bool ok = true;
+  explicit Arg(const at::Tensor& x) : t(x.defined() ? &x : nullptr) {}
   explicit Arg(PyObject* o) {
     if (o == Py_None) return;
     if (!THPVariable_CheckExact(o)) {
@@ -93,6 +94,10 @@ bool table(const Arg& a, int64_t dev, int64_t half) {
 
 bool weight(const Arg& a, int64_t dev, int64_t D) {
   return code_of(a->scalar_type()) >= 0 && on(a, dev) && a->dim() == 1 && a->size(0) == D && a->is_contiguous();
+}
+
+bool positions(const Arg& a, int64_t dev, int64_t B, int64_t S) {
+  return a->scalar_type() == at::kInt && on(a, dev) && a->dim() == 2 && a->size(0) == B && a->size(1) == S;
 }
 
 void seq_strides(int64_t (&to)[3], const at::Tensor& t) {
@@ -204,11 +209,31 @@ struct NormRopeSaved {
   double eps = 0;
 };
 
+// Whether the saved tensors are as the forward took them (but for q's and k's strides): hooks on
+// saved tensors may give back others, also on the host.
+bool as_saved(const NormRopeSaved& a, const variable_list& g) {
+  const Arg q(a.t[0]), k(a.t[1]), qw(a.t[2]), kw(a.t[3]), c(a.t[4]), s(a.t[5]), pos(a.t[6]);
+  if (!q || !k || !q->is_cuda()) return false;
+  const int64_t dev = q->get_device();
+  if (!on(k, dev) || q->dim() != 4 || k->dim() != 4 || code_of(q->scalar_type()) < 0 ||
+      k->scalar_type() != q->scalar_type() || k->size(0) != q->size(0) || k->size(3) != q->size(3) ||
+      bool(qw) != bool(kw) || bool(c) != bool(s))
+    return false;
+  const int64_t D = q->size(3);
+  return (!qw || (weight(qw, dev, D) && weight(kw, dev, D))) &&
+         (!c || (table(c, dev, D / 2) && table(s, dev, D / 2) && c->size(0) == s->size(0))) &&
+         (!pos || (positions(pos, dev, q->size(0), q->size(1)) && k->size(1) == q->size(1))) &&
+         (!g[0].defined() || (g[0].sizes() == q->sizes() && g[0].scalar_type() == q->scalar_type())) &&
+         (!g[1].defined() || (g[1].sizes() == k->sizes() && g[1].scalar_type() == k->scalar_type()));
+}
+
 // Gradients of q, k and the weights from those of the outputs, either of which may be undefined.
 variable_list norm_rope_gradients(const NormRopeSaved& a, variable_list g, bool want_qw, bool want_kw) {
-  const at::Tensor &q = a.t[0], &k = a.t[1], &qw = a.t[2], &kw = a.t[3];
+  if (!as_saved(a, g)) throw std::runtime_error("qk_norm_rope: saved tensors came back changed");
+  auto dense = [](const at::Tensor& t) { return t.stride(3) == 1 ? t : t.contiguous(); };
+  const at::Tensor q = dense(a.t[0]), k = dense(a.t[1]), &qw = a.t[2], &kw = a.t[3];
   for (at::Tensor& t : g)
-    if (t.defined() && t.stride(3) != 1) t = t.contiguous();
+    if (t.defined()) t = dense(t);
   variable_list out(4);
   const c10::OptionalDeviceGuard device(q.device());
   at::AutoDispatchBelowADInplaceOrView below;  // plain allocations
@@ -347,9 +372,7 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (wants_grad(c) || wants_grad(s)) return none();
     for (const Arg* x : {&q, &k, &qw, &kw, &c, &s})
       if (has_tangent(*x)) return none();
-    if (pos && (pos->scalar_type() != at::kInt || !on(pos, dev) || pos->dim() != 2 || pos->size(0) != B ||
-                pos->size(1) != q->size(1) || q->size(1) != k->size(1)))
-      return none();
+    if (pos && !(positions(pos, dev, B, q->size(1)) && q->size(1) == k->size(1))) return none();
     const int64_t offset = PyLong_AsLongLong(a[7]), k_offset = PyLong_AsLongLong(a[8]);
     if (PyErr_Occurred()) return nullptr;
     const double eps = PyFloat_AS_DOUBLE(a[9]);

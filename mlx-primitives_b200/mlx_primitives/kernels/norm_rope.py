@@ -125,6 +125,17 @@ def _forward(dev, q, k, q_weight, k_weight, cos, sin, positions, offset, k_offse
     return q_out, k_out
 
 
+def _as_saved(dev, q, k, q_weight, k_weight, cos, sin, positions, gq, gk) -> bool:
+    """Whether the saved tensors are as the forward took them (but for q's and k's strides): hooks on
+    saved tensors may give back others, also on the host."""
+    return (_quick_ok(q, k, q_weight, k_weight, cos, sin, positions)
+            and q.get_device() == dev and k.get_device() == dev
+            and all(w is None or _lib.plain(w, dev, w.dtype) for w in (q_weight, k_weight))
+            and all(t is None or _lib.plain(t, dev, torch.float32) for t in (cos, sin))
+            and (positions is None or (positions.dtype is torch.int32 and positions.get_device() == dev))
+            and all(g is None or (g.shape == x.shape and g.dtype is x.dtype) for g, x in ((gq, q), (gk, k))))
+
+
 class _QKNormRopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, dev, q, k, q_weight, k_weight, cos, sin, positions, offset, k_offset, eps):
@@ -138,7 +149,9 @@ class _QKNormRopeFn(torch.autograd.Function):
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         dev, offset, k_offset, eps = ctx.args
-        gq, gk = _dense(gq), _dense(gk)
+        if not _as_saved(dev, q, k, q_weight, k_weight, cos, sin, positions, gq, gk):
+            raise RuntimeError("qk_norm_rope: saved tensors came back changed")
+        q, k, gq, gk = _dense(q), _dense(k), _dense(gq), _dense(gk)
         dq = None if gq is None else _lib.rows_like(q)
         dk = None if gk is None else _lib.rows_like(k)
         dqw = torch.empty_like(q_weight) if ctx.needs_input_grad[3] else None

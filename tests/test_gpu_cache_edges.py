@@ -537,3 +537,38 @@ def test_attention_past_32_bits(block):
         q = _rand(rs, (2, Sq, 8, D), torch.bfloat16)
         out = _attend(q, pools, scales, bt, n)
         _check_attn(out, q, [p[near:] for p in pools], [s[near:] for s in scales], bt - near, n)
+
+
+@pytest.mark.parametrize("ints", [torch.int32, torch.int64])  # the node in C++, the one in Python
+def test_norm_rope_with_hooks_on_saved_tensors(ints):
+    """Hooks may move what is saved and give it back in another layout; what comes back on the host,
+    in another type or shape is refused before the kernel sees its address."""
+    from torch.autograd.graph import save_on_cpu, saved_tensors_hooks
+
+    from mlx_primitives.kernels import qk_norm_rope
+    leaves = [t.requires_grad_(True) for t in _norm_case(2, 9, 4, 2, 64, torch.float32)]
+    cos, sin = _tables(16, 32)
+    pos = torch.arange(9, device="cuda").repeat(2, 1).to(ints)
+    rs = np.random.RandomState(53)
+    g = [_rand(rs, t.shape, torch.float32) for t in leaves[:2]]
+
+    def run(hooks=None):
+        if hooks is None:
+            out = qk_norm_rope(*leaves, cos, sin, positions=pos)
+        else:
+            with hooks:
+                out = qk_norm_rope(*leaves, cos, sin, positions=pos)
+        return torch.autograd.grad(out, leaves, g)
+    want = run()
+    same = lambda t: t
+    turned = lambda t: t.transpose(1, 3).contiguous().transpose(1, 3) if t.dim() == 4 else t
+    for hooks in (save_on_cpu(), saved_tensors_hooks(turned, same), saved_tensors_hooks(same, turned)):
+        assert all(torch.equal(a, b) for a, b in zip(run(hooks), want))
+    for back in (lambda t: t.cpu(), lambda t: t.half(), lambda t: t[:1], lambda t: t.repeat_interleave(2, -1)[..., ::2],
+                 lambda t: t if t.dim() == 4 else t.cpu(), lambda t: t if t.dim() != 2 else t.double()):
+        with pytest.raises(RuntimeError, match="came back changed"):
+            run(saved_tensors_hooks(same, back))
+    with saved_tensors_hooks(same, lambda t: t.half()):
+        out = qk_norm_rope(leaves[0], leaves[1], None, None, eps=1e-6 if ints is torch.int32 else 1)
+    with pytest.raises(RuntimeError, match="came back changed"):
+        torch.autograd.grad(out, leaves[:2], g)
