@@ -572,3 +572,14 @@ def test_norm_rope_with_hooks_on_saved_tensors(ints):
         out = qk_norm_rope(leaves[0], leaves[1], None, None, eps=1e-6 if ints is torch.int32 else 1)
     with pytest.raises(RuntimeError, match="came back changed"):
         torch.autograd.grad(out, leaves[:2], g)
+
+
+@pytest.mark.parametrize("H,Hk,Sq,lens", [(64, 4, 17, 1000), (16, 8, 130, 300), (8, 1, 70, 3000), (8, 8, 129, 140)])
+@pytest.mark.parametrize("dtype,kind,D", [("bf16", "e4m3", 64), ("fp16", "int8", 128)])
+def test_attention_of_many_rows_whose_last_tile_is_alone(H, Hk, Sq, lens, dtype, kind, D):
+    """The last 128 and fewer rows of a pool head leave a CTA's second tile without work; units with
+    rows for both follow in the same CTA."""
+    rs = np.random.RandomState(Sq)
+    B = max(3, 20000 // (Sq * H))
+    case = _attn_case(rs, [lens] + rs.randint(1, lens, B - 1).tolist(), H, Hk, D, 16, TYPES[dtype], kind, Sq=Sq)
+    _check_attn(_attend(*case), *case)
