@@ -629,7 +629,9 @@ __global__ void __launch_bounds__(32 * kQaWarps, MINB)
         if (row < p.R && i < r.qlen) qa_row_range(p, r.ctx, r.qlen, i, lo, hi);
         s_lo[threadIdx.x] = lo;
         s_hi[threadIdx.x] = hi;
-        s_pos[threadIdx.x] = (int)(r.ctx - r.qlen + i);
+        // ALiBi counts from the last key that there can be where the position lies behind it: the
+        // softmax does not see the difference, fp32 does
+        s_pos[threadIdx.x] = (int)min(r.ctx - r.qlen + i, (long long)p.max_blocks * p.block_size);
       }
       if (p.alibi && threadIdx.x < HP * ROWS) {
         const int hw = threadIdx.x / ROWS, row = r0 + threadIdx.x % ROWS;

@@ -583,3 +583,19 @@ def test_attention_of_many_rows_whose_last_tile_is_alone(H, Hk, Sq, lens, dtype,
     B = max(3, 20000 // (Sq * H))
     case = _attn_case(rs, [lens] + rs.randint(1, lens, B - 1).tolist(), H, Hk, D, 16, TYPES[dtype], kind, Sq=Sq)
     _check_attn(_attend(*case), *case)
+
+
+@pytest.mark.parametrize("Sq", [1, 5])
+@pytest.mark.parametrize("kw", [dict(), dict(alibi=True), dict(causal=False, alibi=True), dict(window_size=100)])
+def test_attention_of_contexts_longer_than_their_tables(Sq, kw):
+    """Tokens past the block table are not there; the queries' positions still count them."""
+    from mlx_primitives.cache import get_alibi_slopes
+    rs = np.random.RandomState(54)
+    q, pools, scales, bt, _ = _attn_case(rs, [300, 90, 200, 31, 400], 8, 2, 64, 16, torch.bfloat16, "e4m3", Sq=Sq)
+    cap = bt.shape[1] * 16
+    ctx = np.array([300, cap, cap + 3, cap + 10 ** 6, 2 ** 31 - 1], dtype=np.int32)
+    kw = dict(kw)
+    if kw.pop("alibi", False):
+        kw["alibi_slopes"] = get_alibi_slopes(8).numpy()
+    case = (q, pools, scales, bt, ctx)
+    _check_attn(_attend(*case, **kw), *case, **kw)
