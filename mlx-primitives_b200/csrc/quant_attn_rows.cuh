@@ -31,8 +31,8 @@
 // K and V have two stages each in shared memory (64 KB each at D = 128) beside the 64 KB of Q.
 // The scales' ring has four: a group's are written at chunk j + 3 at the earliest after both
 // tiles' weights of chunk j, since K's stage is released by QK(j + 1), which follows PV(j).
-// A tile without rows (the last 128 and fewer of a head's) waits for and releases each stage like
-// the other.  Every mbarrier wait is bounded; after one gave up nothing more is written.
+// A tile without rows (beside the last 128 and fewer of a head's) waits for and releases each stage
+// like the other.  Every mbarrier wait is bounded; after one gave up nothing more is written.
 #pragma once
 
 #include "quant_attn.cuh"
@@ -170,7 +170,9 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
     const uint32_t q_lo = ((sbase + C::OFF_Q + t * C::TILE) >> 4) | (1u << 16);
     const uint32_t k_lo = ((sbase + C::OFF_K) >> 4) | (1u << 16);
     const uint32_t v_lo = ((sbase + C::OFF_V) >> 4) | ((uint32_t)(C::BOX >> 4) << 16);
-    // Scores of the CTA's key tile c, once K is there.  A stage's release counts both tiles.
+    // Scores of the CTA's key tile c, once K is there.  A stage's release counts both tiles; where
+    // no unit has rows for tile 1, tile 0 releases for both.
+    const bool one = p.R <= 128;
     auto issue_qk = [&](int c) {
       const int st = c & 1;
       if (!mbar_wait(BAR(C::B_KF + st), (c >> 1) & 1, wctx, kSiteQuantRows)) return false;
@@ -184,6 +186,7 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
                  sdesc(b + (uint32_t)((kb * C::BOX + kk * 32) >> 4)), idesc_qk, (kb | kk) ? 1u : 0u);
       tc_commit(BAR(C::B_SF + t));
       tc_commit(BAR(C::B_KE + st));
+      if (one) tc_commit(BAR(C::B_KE + st));
       return true;
     };
     auto issue_pv = [&](int c, bool first) {
@@ -195,15 +198,17 @@ __global__ void __launch_bounds__(kQrThreads, 1) quant_attn_rows_kernel(const Qa
       for (int kk = 0; kk < 8; ++kk)
         mma_ts(d_o, d_s + kk * 8, sdesc(b + (uint32_t)(kk * 16 * 128 >> 4)), idesc_pv, (!first || kk > 0) ? 1u : 0u);
       tc_commit(BAR(C::B_VE + st));
+      if (one) tc_commit(BAR(C::B_VE + st));
       return true;
     };
     while (w.f < w.f_end) {
       const Unit u = next_unit();
       if (t >= u.tiles) {
-        // No rows for tile 1, which goes through the stages all the same: a wait by parity tells a
-        // phase from its neighbours only, so that a tile that ran ahead would take a stage of two
-        // chunks before for its own, and one that fell behind would miss a phase.
-        if (issuer) {
+        // No rows for tile 1 here.  If it has some in other units it goes through the stages all the
+        // same: a wait by parity tells a phase from its neighbours only, so that a tile that ran
+        // ahead would take a stage of two chunks before for its own, and one that fell behind would
+        // miss a phase.
+        if (issuer && !one) {
           for (int c = cnt; c < cnt + u.ch1 - u.ch0; ++c) {
             const int st = c & 1;
             if (!mbar_wait(BAR(C::B_KF + st), (c >> 1) & 1, wctx, kSiteQuantRows)) break;
