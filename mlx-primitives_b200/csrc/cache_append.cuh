@@ -4,7 +4,8 @@
 // Token i of sequence b (i < new_lens[b]) has position pos = context_lens[b] + i and goes to row
 // pos % block_size of pool block block_tables[b][pos / block_size].  A position below 0 or past
 // the table, and a table entry outside [0, num_blocks), drop the token; nothing else is written.
-// Queries of dropped or padding tokens become zeros.
+// Queries of padding tokens and of positions outside the table become zeros (one whose block is
+// missing is computed: it may attend to what is there).
 //
 // 16/32-bit pools: the rows are written as computed, rounded once (row units as in norm_rope.cuh,
 // which also describes the norm and the rotation).

@@ -21,10 +21,10 @@ namespace {
 // Query rows a pool head from which the many-row kernel (tcgen05, 256 rows a unit) is taken.  It
 // reads and converts the codes once for all of a unit's rows, the other once for every 16.
 // Measured at 8 heads of 128, e4m3, four contexts of 8 K / 64 of 2 K / one of 1000 tokens:
-//   48 rows   62 us against  82 / 283 against 219 / 19 against 21
-//   64        63 against  92     / 283 against 275 / 19 against 21
-//  128        70 against 147     / 295 against 502 / 21 against 26
-//  256        91 against 254     / 320 against 949 / 27 against 37
+//   48 rows   65 us against  82 / 290 against 220 / 19 against 21
+//   64        65 against  93     / 281 to 294 against 276 / 19 against 21
+//  128        72 against 148     / 290 to 300 against 503 / 21 against 26
+//  256        90 against 254     / 315 to 325 against 956 / 27 against 37
 constexpr int kRowsFrom = 64;
 
 struct QaPlan {
@@ -40,7 +40,11 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // CTAs an SM holds (the launch bounds below are the same numbers).  Three rather than the four
 // that 128 registers a thread allow: four contexts of 128 K tokens 180 us against 190, 48 ragged
-// ones at head_dim 64 35 against 40, at two 239 and 43.
+// ones at head_dim 64 35 against 40, at two 239 and 43.  With two row tiles at head_dim 128 (9 to 63
+// rows a pool head) the 168 registers of three spill (up to 148 bytes a thread stored, 272 loaded),
+// those of two do not; 32 heads over 8 of 128, e4m3, three against two: four contexts of 128 K tokens
+// 259 us against 263 at 16 rows and 657 against 720 at 48, eight of 4 K 52 against 43 and 80 against
+// 76.
 template <int D, int NT, bool SPLIT>
 constexpr int qa_min_ctas() {
   return SPLIT && D == 128 ? 2 : 3;

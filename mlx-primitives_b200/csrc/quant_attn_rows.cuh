@@ -8,7 +8,9 @@
 // them, 1024 cycles); as it stands by the chain that a tile's chunk runs through: scores out of
 // TMEM, maximum, exponentials, weights back, PV, the next QK, 5.5 to 6 K cycles, of which the two
 // tiles hide half.  Four sequences of 512 queries and contexts to 8 K, 32 heads over 8 of 128:
-// 317 to 328 us and 20 for the merge, 525 to 544 TFLOP/s.
+// 344 to 351 us, 20 of them the merge, 521 to 532 TFLOP/s (int8 373).  At head_dim 128 the converting
+// warps spill within their 104 registers (up to 172 bytes a thread stored, 276 loaded): 64 of them
+// are the codes under way.
 //
 // The codes become fp16 (exactly) on their way into shared memory, once for both tiles: the MMA
 // reads 16-bit operands, and 8-bit queries would lose what the cache kept.  Scales stay out of

@@ -235,16 +235,6 @@ class ArgStruct:
         return self._struct.pack(self.size, *fields)
 
 
-def seq_strides(t: torch.Tensor) -> tuple:
-    """Element strides (batch, head, seq) of a (batch, seq, head, dim) tensor."""
-    s = t.stride()
-    return s[0], s[2], s[1]
-
-
-def address(t) -> int:
-    return 0 if t is None else t.data_ptr()
-
-
 # Handle of a device index's current stream, without building a Stream object.
 raw_stream = torch._C._cuda_getCurrentRawStream
 

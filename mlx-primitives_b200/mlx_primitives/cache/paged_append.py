@@ -106,14 +106,15 @@ def paged_append(
     are dropped, as missing blocks are in ``paged_attention``; nothing else is written.  Keys and
     queries are normed with ``k_weight`` / ``q_weight`` and rotated with the tables' rows of their
     positions (each where given; the tables must cover every position of the block tables).
-    Padding rows of q come back as zeros.
+    Rows of q past ``new_lens`` or outside the block table come back as zeros.
 
     Pools: (num_blocks, block_size, kv_heads, head_dim) of k's dtype, or float8_e4m3fn or int8
     with ``k_scales``, ``v_scales`` (num_blocks, kv_heads) float32: value = code * scale.  A
     block's scale is the least power of two that holds its tokens; it is set when the block
     receives its first row and grows, its earlier codes being rescaled, when a later token needs
     it to.  A block that receives tokens must belong to one sequence (full blocks may be shared):
-    the order of two writers of a block is not defined.  Not differentiable.
+    the order of two writers of a block is not defined.  Not differentiable, in either mode; the
+    pools and scales are marked as changed, as by any operator that writes in place.
     """
     out = _lib.calls().append(k, v, k_pool, v_pool, block_tables, context_lens, new_lens, q, cos_cache,
                               sin_cache, q_weight, k_weight, k_scales, v_scales, eps)

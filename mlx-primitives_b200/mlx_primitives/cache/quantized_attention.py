@@ -59,8 +59,9 @@ def quantized_paged_attention(
     (default seq_q); rows behind them come back as zeros, as do rows that see no key.
     ``window_size`` W keeps keys at most W positions away, as ``sliding_window_attention`` does.
     ALiBi adds slope[h] * (key position - query position).  Returns q's shape and dtype.  Rows and
-    blocks behind the contexts may hold anything; a NaN or infinity among a sequence's own values
-    may reach all its rows, also those that do not see it.  Not differentiable.
+    blocks behind the contexts or before every query's window may hold anything; a NaN or infinity
+    that some query sees may reach all its sequence's rows, also those that do not see it.  Not
+    differentiable, in either mode.
     """
     if alibi_slopes is None and (window_size is None or window_size >= 0):
         out = _lib.calls().attend(q, k_pool, v_pool, k_scales, v_scales, block_tables, context_lens,

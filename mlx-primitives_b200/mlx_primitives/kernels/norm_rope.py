@@ -8,8 +8,9 @@ position and r = (mean(x^2) + eps)^(-1/2):
     y = x * r * weight
     out[..., :h] = y[..., :h] * cos[p] - y[..., h:] * sin[p]
     out[..., h:] = y[..., :h] * sin[p] + y[..., h:] * cos[p].
-Computed in fp32 and rounded once.  Differentiable in q, k and the weights (mlxp_qk_norm_rope_bwd);
-the weights' gradients are summed in fp32 in a fixed order, so every run gives the same bits.
+Computed in fp32 and rounded once.  Differentiable in q, k and the weights, in reverse mode and
+once (mlxp_qk_norm_rope_bwd); the weights' gradients are summed in fp32 in a fixed order, so every
+run gives the same bits.
 """
 
 from __future__ import annotations
