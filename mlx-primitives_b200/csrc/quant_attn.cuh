@@ -17,9 +17,9 @@
 //
 // How the codes get there.  Where the block size is a multiple of 16 a tile is one TMA box of K
 // and one of V (16 rows of one head), three or four stages in flight a warp, each on its own
-// mbarrier.  Four contexts of 128 K tokens, 8 heads of 128 (1.07 GB of codes): 179 to 186 us in a row
-// of calls, 92 to 89 % of the measured HBM rate, 10 of them the merge; a call by itself behind a flush
-// of L2 196 to 199.  Four CTAs an SM instead of three 190 us, loads into registers 257 (a warp is
+// mbarrier.  Four contexts of 128 K tokens, 8 heads of 128 (1.07 GB of codes): 179 to 186 us where
+// two sets of tensors take turns, 92 to 89 % of the measured HBM rate, 10 of them the merge; 196 to 201
+// behind a flush of L2 or on new tensors each time.  Four CTAs an SM instead of three 190 us, loads into registers 257 (a warp is
 // then one tile ahead), cp.async 284 (28 instructions a tile keep the load path busy).  Eight of 4 K,
 // 32 heads (269 MB): 52 us and 5 for the merge.  Other block sizes do take cp.async, every lane
 // copying the bytes that it reads itself (blocks of 24: 310 us at 128 K).  The order of a dot
