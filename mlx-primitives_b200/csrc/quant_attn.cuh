@@ -18,11 +18,12 @@
 // How the codes get there.  Where the block size is a multiple of 16 a tile is one TMA box of K
 // and one of V (16 rows of one head), three or four stages in flight a warp, each on its own
 // mbarrier.  Four contexts of 128 K tokens, 8 heads of 128 (1.07 GB of codes): 179 to 186 us where
-// two sets of tensors take turns, 92 to 89 % of the measured HBM rate, 10 of them the merge; 196 to 201
-// behind a flush of L2 or on new tensors each time.  Four CTAs an SM instead of three 190 us, loads into registers 257 (a warp is
-// then one tile ahead), cp.async 284 (28 instructions a tile keep the load path busy).  Eight of 4 K,
-// 32 heads (269 MB): 52 us and 5 for the merge.  Other block sizes do take cp.async, every lane
-// copying the bytes that it reads itself (blocks of 24: 310 us at 128 K).  The order of a dot
+// two sets of tensors take turns, 92 to 89 % of the measured HBM rate, 10 of them the merge; 196 to
+// 201 behind a flush of L2 or on new tensors each time.  Four CTAs an SM instead of three 190 us,
+// loads into registers 257 (a warp is then one tile ahead), cp.async 284 (28 instructions a tile
+// keep the load path busy).  Eight of 4 K, 32 heads (269 MB): 52 us and 5 for the merge.  Other block
+// sizes do take cp.async, every lane copying the bytes that it reads itself (blocks of 24: 310 us at
+// 128 K).  The order of a dot
 // product's terms is free, so the fragments are filled straight from the rows: of a K row the four
 // lanes c of a row group hold 16-byte pieces, each word of which is one k16 step's two pairs; of a
 // V row the eight lanes g hold D / 8 bytes each, and a byte permute of two keys' words gives the
